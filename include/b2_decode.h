@@ -70,6 +70,7 @@ typedef enum b2_dtype { B2_F32 = 0, B2_F16 = 1, B2_BF16 = 2 } b2_dtype;
 #define B2_DEVERR_SEQ_LEN 2u    /* a seq_len beyond max_blocks_per_seq*16 (or < 0) was clamped */
 #define B2_DEVERR_TIMEOUT 4u    /* a bounded pipeline wait gave up; the output is invalid */
 #define B2_DEVERR_TOKEN 8u      /* a token id or position outside its table was clamped */
+#define B2_DEVERR_NO_BLOCKS 16u /* b2_block_map: the free list did not cover a sequence; it got no rows */
 
 /* Library version string. */
 B2_API const char* b2_version(void);
@@ -468,6 +469,185 @@ typedef struct B2LmHeadArgmaxArgs {
 
 B2_API size_t b2_lm_head_argmax_workspace_bytes(int32_t batch);
 B2_API int b2_lm_head_argmax(const B2LmHeadArgmaxArgs* args, b2_stream_t stream);
+
+/* ------------------------------------------------------------------ block tables and slots on the device
+ * The block bookkeeping of one step for callers that keep lengths and block
+ * tables on the GPU (a decode loop in a CUDA graph, without a host round
+ * trip).  No reference counterpart on the device: the reference allocates on
+ * the host (BlockPool / BlockTable, gpu-engine/include/engine/kv_cache.h:16-57)
+ * and uploads the tables every step.  The policy is the same: a LIFO stack of
+ * free ids, free_list[0 .. free_count - 1], whose top is handed out first.
+ *
+ * b2_block_map gives every sequence b the blocks that its new_lens[b] rows
+ * need beyond the ceil(seq_lens_pre[b] / 16) it has, in order of b and then of
+ * position, and maps each row to its slot.  With
+ * q_start[b] = new_lens[0] + .. + new_lens[b - 1], row q_start[b] + i is
+ * position p = seq_lens_pre[b] + i of sequence b, and
+ *   slots[q_start[b] + i] = block_tables[b][p / 16] * 16 + p % 16.
+ * Rows behind the last sequence's (up to max_rows) get slot -1, which
+ * b2_kv_append_q4 and b2_kv_gather_q4 skip.  New table entries are written
+ * into block_tables; no other entry is touched.  Only the entries of blocks a
+ * sequence already has need to be valid on entry.
+ *
+ * A sequence is refused -- slots -1, seq_lens_post = seq_lens_pre, no block
+ * taken -- when it needs blocks and the list does not cover the need of all
+ * sequences up to and including it (B2_DEVERR_NO_BLOCKS), when a length is
+ * negative, seq_lens_pre + new_lens > max_blocks_per_seq * 16, or its rows end past
+ * max_rows (B2_DEVERR_SEQ_LEN).  Its rows still count in q_start (a negative
+ * new_lens as none), capped at max_rows.  A block id outside [0, num_blocks)
+ * sets B2_DEVERR_BLOCK_ID and its rows get slot -1; a free_count outside
+ * [0, num_blocks] is clamped into it with the same bit.
+ *
+ * seq_lens_post may be seq_lens_pre and free_count_out may be free_count
+ * (in place); no other two arrays may overlap.  n_seqs <= B2_MAP_MAX_SEQS,
+ * slots 16-byte aligned.  One launch of one thread-block cluster. */
+#define B2_MAP_MAX_SEQS 16384
+
+typedef struct B2BlockMapArgs {
+    int32_t n_seqs;
+    int32_t max_blocks_per_seq;
+    int32_t num_blocks;            /* pool capacity; free_list has room for as many ids */
+    int32_t max_rows;              /* entries of slots */
+    const int32_t* seq_lens_pre;   /* [n_seqs] */
+    const int32_t* new_lens;       /* [n_seqs], or NULL: one row each (a decode step) */
+    const int32_t* free_list;      /* [num_blocks] */
+    const int32_t* free_count;     /* [1] */
+    int32_t* block_tables;         /* [n_seqs, max_blocks_per_seq], updated */
+    int32_t* slots;                /* [max_rows] output */
+    int32_t* q_start;              /* optional [n_seqs] output */
+    int32_t* seq_lens_post;        /* optional [n_seqs] output */
+    int32_t* free_count_out;       /* [1] output */
+} B2BlockMapArgs;
+
+B2_API int b2_block_map(const B2BlockMapArgs* args, b2_stream_t stream);
+
+/* Gives back the ceil(seq_lens[b] / 16) blocks of every sequence with
+ * release[b] != 0: their ids go on top of the free list in order of b and then
+ * of position, seq_lens_out[b] becomes 0 (other sequences' lengths are
+ * copied), and free_count_out = free_count + the ids given back.  Replaces
+ * BlockPool::free over a sequence's table (gpu-engine/src/kv_cache_pool.cpp:18-28)
+ * for tables that live on the device.  Table entries are not cleared.  A
+ * block must belong to one sequence only.  An id outside [0, num_blocks) sets
+ * B2_DEVERR_BLOCK_ID and is left out; ids that would go past num_blocks entries
+ * (something was given back twice) set it too and are dropped.  A seq_len
+ * outside [0, max_blocks_per_seq * 16] is clamped into it and sets
+ * B2_DEVERR_SEQ_LEN.  seq_lens_out may be seq_lens, free_count_out may be
+ * free_count; no other two arrays may overlap.  n_seqs <= B2_MAP_MAX_SEQS.
+ * One launch of one thread-block cluster. */
+typedef struct B2BlockReleaseArgs {
+    int32_t n_seqs;
+    int32_t max_blocks_per_seq;
+    int32_t num_blocks;
+    const int32_t* block_tables; /* [n_seqs, max_blocks_per_seq] */
+    const int32_t* seq_lens;     /* [n_seqs] */
+    const int32_t* release;      /* [n_seqs] */
+    int32_t* free_list;          /* [num_blocks], entries from free_count on are written */
+    const int32_t* free_count;   /* [1] */
+    int32_t* free_count_out;     /* [1] output */
+    int32_t* seq_lens_out;       /* optional [n_seqs] output */
+} B2BlockReleaseArgs;
+
+B2_API int b2_block_release(const B2BlockReleaseArgs* args, b2_stream_t stream);
+
+/* ------------------------------------------------------------------ 4-bit KV cache
+ * A paged pool whose rows are held in 4 bits: 1.25 * head_dim bytes for a
+ * token's K and V of one kv head, against 4 * head_dim in 16 bits.  No
+ * reference counterpart (its pool is f16 only).  Each group of 32 head dims of
+ * one token's K or V row has a scale s and a middle m in f16 and a 4-bit code per
+ * element:
+ *   s = f16((max - min) / 15),  m = f16(min + 8 s),
+ *   c = clamp(round_to_nearest_even((x - m) / s) + 8, 0, 15)   (8 where s = 0),
+ * and the element reads back as s * (c - 8) + m.  x is clamped to +-65504
+ * first; a group that holds a NaN or an infinity stores NaN for s and m and
+ * reads back as NaN.
+ *
+ * Layout: [block][layer][n_kv_head] chunks of 20 * head_dim bytes, each 16
+ * token positions of one kv head; with G = head_dim / 32,
+ *   K codes  [16][4][G] 32-bit words: word (i, g) holds dims 32 g + 8 i + j,
+ *            j = 0..7 from the low nibble up
+ *   K params [16][G] 32-bit words: m in the low half, s in the high half
+ *   V codes  [head_dim / 64][16][16 / G][G] 16-bit units: unit (plane, t, r, g)
+ *            holds dims 32 g + 4 (plane * 16 / G + r) + j, j = 0..3
+ *   V params like K's.
+ * head_dim is 64 or 128.  b2_kv_q4_pool_bytes gives the pool's size (0 for
+ * shapes that are refused).  The pool needs no initialisation.
+ *
+ * b2_kv_append_q4 quantises rows of k and v ([rows][row_stride], head h at
+ * columns h * head_dim, F16 or BF16) into the slots of layer layer_idx;
+ * b2_kv_gather_q4 writes the values of those slots into k and v (rounded once
+ * to dtype).  slot = block * 16 + position in the block.  A row with a negative
+ * slot is skipped: the append writes nothing, the gather leaves the row of k
+ * and v as it is.  A slot >= 16 * num_blocks is skipped too and sets
+ * B2_DEVERR_BLOCK_ID.  The slots of one append must differ (two rows with one
+ * slot leave a mixture of the two in it); a gather may name a slot repeatedly.
+ * k, v and the pool are 16-byte aligned, row_stride a multiple of 8 elements. */
+typedef struct B2KvQ4Args {
+    int32_t dtype;        /* B2_F16 or B2_BF16, for k and v */
+    void* kv_pool;
+    void* k;              /* read by the append, written by the gather */
+    void* v;
+    int64_t row_stride;   /* elements between rows of k and of v */
+    const int32_t* slots; /* [rows] */
+    int32_t rows;
+    int32_t n_kv_head;
+    int32_t head_dim;     /* 64 or 128 */
+    int32_t layer_idx;
+    int32_t n_layer;
+    int32_t num_blocks;   /* pool capacity in blocks */
+} B2KvQ4Args;
+
+B2_API size_t b2_kv_q4_pool_bytes(int32_t num_blocks, int32_t n_layer, int32_t n_kv_head, int32_t head_dim);
+B2_API int b2_kv_append_q4(const B2KvQ4Args* args, b2_stream_t stream);
+B2_API int b2_kv_gather_q4(const B2KvQ4Args* args, b2_stream_t stream);
+
+/* Decode attention over a 4-bit pool, one query token per sequence.  With
+ * n = seq_lens[b] (post-append count) and the query at position n - 1, keys
+ * first <= j < n are visible, where first = max(0, key_starts[b],
+ * n - window if window > 0):
+ *   x_j = scale * q . k_j;  softcap > 0: x_j = softcap * tanh(x_j / softcap)
+ *   alibi_slopes: x_j += alibi_slopes[h] * (j - (n - 1))
+ *   out[b, h, :] = sum_j softmax_j(x) v_j
+ * key_starts masks the keys in front of the query's own document (or a
+ * left-padded batch's padding).  A sequence without visible keys gets zeros.
+ * q and out F16 or BF16 (out also F32); any n_head / n_kv_head from 1 to 8.
+ * A seq_len beyond max_blocks_per_seq * 16 or below 0 is clamped
+ * (B2_DEVERR_SEQ_LEN), a block id outside the pool is clamped
+ * (B2_DEVERR_BLOCK_ID).
+ *
+ * The work is split evenly over the GPU by blocks; partial results meet in
+ * the workspace.  Size it with b2_paged_attention_q4_workspace_bytes and zero it
+ * once; every launch leaves its counters at zero (zero it again after
+ * B2_DEVERR_TIMEOUT).  Launches that may overlap need a workspace each --
+ * captured graphs that may run at the same time included. */
+typedef struct B2PagedAttnQ4Args {
+    int32_t dtype;     /* B2_F16 or B2_BF16: q */
+    int32_t out_dtype; /* B2_F32, or the same as dtype */
+    const void* q;
+    int64_t q_row_stride; /* elements between batch rows of q, a multiple of 8 */
+    const void* kv_pool;
+    const int32_t* block_tables; /* [batch, max_blocks_per_seq] */
+    const int32_t* seq_lens;     /* [batch] */
+    const int32_t* key_starts;   /* optional [batch] */
+    const float* alibi_slopes;   /* optional [n_head] */
+    void* out;                   /* [batch, n_head, head_dim] packed */
+    int32_t batch;
+    int32_t n_head;
+    int32_t n_kv_head;
+    int32_t head_dim; /* 64 or 128 */
+    int32_t max_blocks_per_seq;
+    int32_t layer_idx;
+    int32_t n_layer;
+    int32_t num_blocks;
+    float scale;      /* 0 selects 1/sqrt(head_dim) */
+    float softcap;    /* 0: none */
+    int32_t window;   /* 0: none */
+    int32_t max_ctas; /* 0: the whole GPU; n > 0: at most n CTAs */
+} B2PagedAttnQ4Args;
+
+/* 0 where the arguments are refused (b2_last_error_string says why). */
+B2_API size_t b2_paged_attention_q4_workspace_bytes(const B2PagedAttnQ4Args* args);
+B2_API int b2_paged_attention_q4(const B2PagedAttnQ4Args* args, void* workspace, size_t workspace_bytes,
+                                 b2_stream_t stream);
 
 #ifdef __cplusplus
 }

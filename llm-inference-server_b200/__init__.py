@@ -25,7 +25,7 @@ BLOCK_TOKENS = 16
 B2_OK = 0
 ATTN_INPUTS_READY, ATTN_NEWEST_ROW_PENDING = 1, 2  # B2PagedAttnArgs.flags
 LINEAR_STORE, LINEAR_GELU = 0, 1  # B2LinearArgs.epilogue
-DEVERR_BLOCK_ID, DEVERR_SEQ_LEN, DEVERR_TIMEOUT, DEVERR_TOKEN = 1, 2, 4, 8
+DEVERR_BLOCK_ID, DEVERR_SEQ_LEN, DEVERR_TIMEOUT, DEVERR_TOKEN, DEVERR_NO_BLOCKS = 1, 2, 4, 8, 16
 
 # Every symbol include/b2_decode.h declares.
 DECODE_SYMBOLS = (
@@ -36,6 +36,8 @@ DECODE_SYMBOLS = (
     "b2_tp_epoch_bump", "b2_linear", "b2_prefill_attention", "b2_paged_attention_host",
     "b2_tp_barrier_timed", "b2_device_error_word", "b2_raise_device_error",
     "b2_lm_head_argmax_workspace_bytes", "b2_lm_head_argmax",
+    "b2_block_map", "b2_block_release", "b2_kv_q4_pool_bytes", "b2_kv_append_q4", "b2_kv_gather_q4",
+    "b2_paged_attention_q4_workspace_bytes", "b2_paged_attention_q4",
 )
 
 _c_int, _c_float, _vp = ctypes.c_int32, ctypes.c_float, ctypes.c_void_p
@@ -79,6 +81,33 @@ class PrefillAttnArgs(ctypes.Structure):
                 ("out_row_stride", _c_int), ("n_seqs", _c_int), ("n_head", _c_int), ("n_kv_head", _c_int),
                 ("head_dim", _c_int), ("max_blocks_per_seq", _c_int), ("layer_idx", _c_int), ("n_layer", _c_int),
                 ("num_blocks", _c_int), ("max_q_len", _c_int), ("scale", _c_float)]
+
+
+class BlockMapArgs(ctypes.Structure):
+    _fields_ = [("n_seqs", _c_int), ("max_blocks_per_seq", _c_int), ("num_blocks", _c_int), ("max_rows", _c_int),
+                ("seq_lens_pre", _vp), ("new_lens", _vp), ("free_list", _vp), ("free_count", _vp),
+                ("block_tables", _vp), ("slots", _vp), ("q_start", _vp), ("seq_lens_post", _vp),
+                ("free_count_out", _vp)]
+
+
+class BlockReleaseArgs(ctypes.Structure):
+    _fields_ = [("n_seqs", _c_int), ("max_blocks_per_seq", _c_int), ("num_blocks", _c_int), ("block_tables", _vp),
+                ("seq_lens", _vp), ("release", _vp), ("free_list", _vp), ("free_count", _vp), ("free_count_out", _vp),
+                ("seq_lens_out", _vp)]
+
+
+class KvQ4Args(ctypes.Structure):
+    _fields_ = [("dtype", _c_int), ("kv_pool", _vp), ("k", _vp), ("v", _vp), ("row_stride", ctypes.c_int64),
+                ("slots", _vp), ("rows", _c_int), ("n_kv_head", _c_int), ("head_dim", _c_int), ("layer_idx", _c_int),
+                ("n_layer", _c_int), ("num_blocks", _c_int)]
+
+
+class PagedAttnQ4Args(ctypes.Structure):
+    _fields_ = [("dtype", _c_int), ("out_dtype", _c_int), ("q", _vp), ("q_row_stride", ctypes.c_int64),
+                ("kv_pool", _vp), ("block_tables", _vp), ("seq_lens", _vp), ("key_starts", _vp), ("alibi_slopes", _vp),
+                ("out", _vp), ("batch", _c_int), ("n_head", _c_int), ("n_kv_head", _c_int), ("head_dim", _c_int),
+                ("max_blocks_per_seq", _c_int), ("layer_idx", _c_int), ("n_layer", _c_int), ("num_blocks", _c_int),
+                ("scale", _c_float), ("softcap", _c_float), ("window", _c_int), ("max_ctas", _c_int)]
 
 
 class B2Error(RuntimeError):
@@ -130,6 +159,15 @@ def load() -> ctypes.CDLL:
     lib.b2_tp_epoch_bump.argtypes = [_vp, _vp]
     lib.b2_device_error_word.argtypes = [ctypes.POINTER(ctypes.c_void_p)]
     lib.b2_raise_device_error.argtypes = [ctypes.c_uint32, _vp]
+    lib.b2_block_map.argtypes = [ctypes.POINTER(BlockMapArgs), _vp]
+    lib.b2_block_release.argtypes = [ctypes.POINTER(BlockReleaseArgs), _vp]
+    lib.b2_kv_q4_pool_bytes.argtypes = [_c_int] * 4
+    lib.b2_kv_q4_pool_bytes.restype = ctypes.c_size_t
+    lib.b2_kv_append_q4.argtypes = [ctypes.POINTER(KvQ4Args), _vp]
+    lib.b2_kv_gather_q4.argtypes = [ctypes.POINTER(KvQ4Args), _vp]
+    lib.b2_paged_attention_q4_workspace_bytes.argtypes = [ctypes.POINTER(PagedAttnQ4Args)]
+    lib.b2_paged_attention_q4_workspace_bytes.restype = ctypes.c_size_t
+    lib.b2_paged_attention_q4.argtypes = [ctypes.POINTER(PagedAttnQ4Args), _vp, ctypes.c_size_t, _vp]
     _lib = lib
     return lib
 
@@ -295,3 +333,144 @@ def prefill_attention(out, q, q_row_stride, kv_pool, block_tables, seq_lens_pre,
                         seq_lens_pre.numel(), n_head, n_kv_head, head_dim, max_blocks_per_seq, layer_idx, n_layer,
                         num_blocks, max_q_len, scale)
     _check(load().b2_prefill_attention(ctypes.byref(a), _stream(stream)))
+
+
+# ------------------------------------------------------- block maps and the 4-bit KV cache
+
+def _on_device(args, *tensors):
+    """args, which keeps the tensors it points into alive; they must lie on the current CUDA device,
+    whose streams and workspaces the launch uses."""
+    import torch
+    for t in tensors:
+        if t is not None and not (t.is_cuda and t.device.index == torch.cuda.current_device()):
+            raise ValueError(f"a tensor is on {t.device}, not on the current CUDA device")
+    args.tensors = tensors
+    return args
+
+
+def _int32(name, t, count=None):
+    import torch
+    if t.dtype != torch.int32 or not t.is_contiguous() or (count is not None and t.numel() < count):
+        raise ValueError(f"{name} must be a contiguous int32 tensor" + (f" of at least {count} entries" if count else ""))
+    return t
+
+
+def _q4_pool(pool, num_blocks, n_layer, n_kv_head, head_dim):
+    need = load().b2_kv_q4_pool_bytes(num_blocks, n_layer, n_kv_head, head_dim)
+    if need and (not pool.is_contiguous() or pool.numel() * pool.element_size() < need):
+        raise ValueError(f"the 4-bit pool must be contiguous and hold {need} bytes")
+
+
+def block_map_args(block_tables, seq_lens_pre, free_list, free_count, slots, *, num_blocks, new_lens=None, q_start=None,
+                   seq_lens_post=None, free_count_out=None) -> BlockMapArgs:
+    """Arguments of block_map.  free_count_out=None updates free_count in place."""
+    n, mbps = block_tables.shape
+    for name, t, c in (("block_tables", block_tables, None), ("seq_lens_pre", seq_lens_pre, n), ("slots", slots, None),
+                       ("free_list", free_list, 1), ("free_count", free_count, 1), ("new_lens", new_lens, n),
+                       ("q_start", q_start, n), ("seq_lens_post", seq_lens_post, n), ("free_count_out", free_count_out, 1)):
+        if t is not None:
+            _int32(name, t, c)
+    free_count_out = free_count if free_count_out is None else free_count_out
+    a = BlockMapArgs(n, mbps, num_blocks, slots.numel(), _ptr(seq_lens_pre), _ptr(new_lens), _ptr(free_list),
+                     _ptr(free_count), _ptr(block_tables), _ptr(slots), _ptr(q_start), _ptr(seq_lens_post),
+                     _ptr(free_count_out))
+    return _on_device(a, block_tables, seq_lens_pre, new_lens, free_list, free_count, slots, q_start, seq_lens_post,
+                      free_count_out)
+
+
+def block_map(args: BlockMapArgs, stream=None) -> None:
+    """Blocks for each sequence's new rows from the device free list, and the
+    slot of every row (b2_block_map; the reference's BlockPool allocates on the
+    host, kv_cache.h:16-57)."""
+    _check(load().b2_block_map(ctypes.byref(args), _stream(stream)))
+
+
+def block_release_args(block_tables, seq_lens, release, free_list, free_count, *, num_blocks, seq_lens_out=None,
+                       free_count_out=None) -> BlockReleaseArgs:
+    """Arguments of block_release.  free_count_out=None updates free_count in place."""
+    n, mbps = block_tables.shape
+    for name, t, c in (("block_tables", block_tables, None), ("seq_lens", seq_lens, n), ("release", release, n),
+                       ("free_list", free_list, num_blocks), ("free_count", free_count, 1),
+                       ("seq_lens_out", seq_lens_out, n), ("free_count_out", free_count_out, 1)):
+        if t is not None:
+            _int32(name, t, c)
+    free_count_out = free_count if free_count_out is None else free_count_out
+    a = BlockReleaseArgs(n, mbps, num_blocks, _ptr(block_tables), _ptr(seq_lens), _ptr(release), _ptr(free_list),
+                         _ptr(free_count), _ptr(free_count_out), _ptr(seq_lens_out))
+    return _on_device(a, block_tables, seq_lens, release, free_list, free_count, free_count_out, seq_lens_out)
+
+
+def block_release(args: BlockReleaseArgs, stream=None) -> None:
+    """The blocks of released sequences go back on the device free list (b2_block_release)."""
+    _check(load().b2_block_release(ctypes.byref(args), _stream(stream)))
+
+
+def kv_q4_pool(num_blocks, *, n_layer, n_kv_head, head_dim, device=None):
+    """An uninitialised 4-bit pool, uint8 [num_blocks, n_layer, n_kv_head, 20 * head_dim]."""
+    import torch
+    if load().b2_kv_q4_pool_bytes(num_blocks, n_layer, n_kv_head, head_dim) == 0:
+        raise B2Error(-3, load().b2_last_error_string().decode())
+    return torch.empty(num_blocks, n_layer, n_kv_head, 20 * head_dim, dtype=torch.uint8,
+                       device=device if device is not None else "cuda")
+
+
+def kv_q4_args(kv_pool, k, v, slots, *, n_kv_head, head_dim, layer_idx, n_layer, num_blocks) -> KvQ4Args:
+    """Arguments of kv_append_q4 and kv_gather_q4.  k and v: [rows, n_kv_head, head_dim] or
+    [rows, n_kv_head * head_dim], rows may be strided (both alike)."""
+    rows = slots.numel()
+    _int32("slots", slots)
+    _q4_pool(kv_pool, num_blocks, n_layer, n_kv_head, head_dim)
+    for t in (k, v):
+        if t.shape[0] != rows or t[0:1].numel() != (n_kv_head * head_dim if rows else 0) or t.dtype != k.dtype \
+                or (rows > 0 and not t[0].is_contiguous()) or t.stride(0) != k.stride(0):
+            raise ValueError("k and v must have slots.numel() rows of n_kv_head * head_dim contiguous elements, one dtype and row stride")
+    a = KvQ4Args(dtype_code(k.dtype), _ptr(kv_pool), _ptr(k), _ptr(v), k.stride(0), _ptr(slots), rows, n_kv_head, head_dim,
+                 layer_idx, n_layer, num_blocks)
+    return _on_device(a, kv_pool, k, v, slots)
+
+
+def kv_append_q4(args: KvQ4Args, stream=None) -> None:
+    """Rows of k and v, quantised to 4 bits, into their slots of the pool (b2_kv_append_q4)."""
+    _check(load().b2_kv_append_q4(ctypes.byref(args), _stream(stream)))
+
+
+def kv_gather_q4(args: KvQ4Args, stream=None) -> None:
+    """The values of the pool's slots into rows of k and v (b2_kv_gather_q4)."""
+    _check(load().b2_kv_gather_q4(ctypes.byref(args), _stream(stream)))
+
+
+def attn_q4_args(q, kv_pool, block_tables, seq_lens, out, *, n_head, n_kv_head, head_dim, layer_idx, n_layer, num_blocks,
+                 scale=0.0, softcap=0.0, window=0, key_starts=None, alibi_slopes=None, max_ctas=0) -> PagedAttnQ4Args:
+    """Arguments of paged_attention_q4.  q: [batch, n_head, head_dim] or [batch, n_head * head_dim], rows may be strided."""
+    import torch
+    batch, mbps = block_tables.shape
+    _q4_pool(kv_pool, num_blocks, n_layer, n_kv_head, head_dim)
+    for name, t, c in (("block_tables", block_tables, None), ("seq_lens", seq_lens, batch), ("key_starts", key_starts, batch)):
+        if t is not None:
+            _int32(name, t, c)
+    if q.shape[0] != batch or (batch > 0 and (q[0].numel() != n_head * head_dim or not q[0].is_contiguous())):
+        raise ValueError("q must have a row of n_head * head_dim contiguous elements for every sequence")
+    if out.numel() != batch * n_head * head_dim or not out.is_contiguous():
+        raise ValueError("out must be contiguous, [batch, n_head, head_dim]")
+    if alibi_slopes is not None and (alibi_slopes.dtype != torch.float32 or alibi_slopes.numel() != n_head
+                                     or not alibi_slopes.is_contiguous()):
+        raise ValueError("alibi_slopes must be float32 [n_head]")
+    a = PagedAttnQ4Args(dtype_code(q.dtype), dtype_code(out.dtype), _ptr(q), q.stride(0), _ptr(kv_pool),
+                        _ptr(block_tables), _ptr(seq_lens), _ptr(key_starts), _ptr(alibi_slopes), _ptr(out), batch,
+                        n_head, n_kv_head, head_dim, mbps, layer_idx, n_layer, num_blocks, scale, softcap, window,
+                        max_ctas)
+    return _on_device(a, q, kv_pool, block_tables, seq_lens, key_starts, alibi_slopes, out)
+
+
+def attention_q4_workspace(args: PagedAttnQ4Args, device=None):
+    """A zeroed workspace for launches shaped like args (every launch leaves its counters at zero)."""
+    import torch
+    n = load().b2_paged_attention_q4_workspace_bytes(ctypes.byref(args))
+    if n == 0:
+        raise B2Error(-3, load().b2_last_error_string().decode() or "workspace size query failed")
+    return torch.zeros(n, dtype=torch.uint8, device=device if device is not None else "cuda")
+
+
+def paged_attention_q4(args: PagedAttnQ4Args, workspace, stream=None) -> None:
+    """Decode attention over the 4-bit pool (b2_paged_attention_q4)."""
+    _check(load().b2_paged_attention_q4(ctypes.byref(args), workspace.data_ptr(), workspace.numel(), _stream(stream)))

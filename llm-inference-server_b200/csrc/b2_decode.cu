@@ -22,8 +22,11 @@
 
 #include "append.cuh"
 #include "attention.cuh"
+#include "attention_q4.cuh"
 #include "attention_tc.cuh"
 #include "b2_common.cuh"
+#include "blocks.cuh"
+#include "kv_q4.cuh"
 #include "linear_tc.cuh"
 #include "lm_head_tc.cuh"
 #include "prefill_tc.cuh"
@@ -1562,3 +1565,194 @@ extern "C" int b2_prefill_attention(const B2PrefillAttnArgs* a, b2_stream_t stre
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return a->dtype == B2_F16 ? launch_prefill_t<__half>(a, pp, map, s) : launch_prefill_t<__nv_bfloat16>(a, pp, map, s);
 }
+
+// ------------------------------------------- block maps and the 4-bit KV cache
+
+namespace b2 {
+namespace {
+
+// Cluster kernels of blocks.cuh: shared bytes above the default need the opt-in.
+template <typename K, typename P>
+int launch_blocks(K kern, std::atomic<uint64_t>& smem_set, int smem, const P& prm, cudaStream_t stream) {
+    int dev = -1;
+    const DeviceInfo di = device_info(&dev);
+    if (dev < 0) return fail(B2_ERR_DEVICE, "no current CUDA device");
+    // The limit, less the kernels' static shared memory.
+    const int rc = ensure_max_smem(kern, smem_set, dev, di.max_smem_optin - 1024);
+    if (rc != B2_OK) return rc;
+    return launch_pdl(kern, dim3(kMapCluster), dim3(kMapThreads), smem, stream, prm);
+}
+
+// The largest slot is below 2^31, and the chunk index (block, layer, head) too.
+int check_q4_shape(int num_blocks, int n_layer, int n_kv_head, int head_dim) {
+    if (head_dim != 64 && head_dim != 128) return fail(B2_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+    if (num_blocks <= 0 || n_layer <= 0 || n_kv_head <= 0)
+        return fail(B2_ERR_SHAPE, "num_blocks, n_layer and n_kv_head must be positive");
+    if (num_blocks > (1 << 27) - 1 || static_cast<double>(num_blocks) * n_layer * n_kv_head >= 2147483648.0)
+        return fail(B2_ERR_SHAPE, "num_blocks must stay below 2^27 and num_blocks*n_layer*n_kv_head below 2^31");
+    return B2_OK;
+}
+
+template <bool kAppend>
+int kv_q4(const B2KvQ4Args* a, b2_stream_t stream) {
+    if (a == nullptr) return fail(B2_ERR_NULL, "args is NULL");
+    if (a->dtype != B2_F16 && a->dtype != B2_BF16) return fail(B2_ERR_DTYPE, "the 4-bit pool takes F16 and BF16 rows");
+    if (a->rows < 0) return fail(B2_ERR_SHAPE, "rows < 0");
+    const int rc = check_q4_shape(a->num_blocks, a->n_layer, a->n_kv_head, a->head_dim);
+    if (rc != B2_OK) return rc;
+    if (a->layer_idx < 0 || a->layer_idx >= a->n_layer) return fail(B2_ERR_SHAPE, "layer_idx out of range");
+    if (a->rows == 0) return B2_OK;
+    if (!a->kv_pool || !a->k || !a->v || !a->slots) return fail(B2_ERR_NULL, "kv_pool, k, v and slots are required");
+    if (a->row_stride < static_cast<int64_t>(a->n_kv_head) * a->head_dim)
+        return fail(B2_ERR_SHAPE, "row_stride < n_kv_head*head_dim");
+    if (!aligned16(a->kv_pool) || !aligned16(a->k) || !aligned16(a->v) || a->row_stride % 8 != 0)
+        return fail(B2_ERR_ALIGN, "pool, k and v must be 16-byte aligned, row_stride a multiple of 8");
+    KvQ4Params p{static_cast<uint8_t*>(a->kv_pool), a->k, a->v, a->row_stride, a->slots, a->rows,
+                 a->n_kv_head, a->layer_idx, a->n_layer, a->num_blocks};
+    const long long total = 2ll * a->rows * a->n_kv_head * (a->head_dim / 8);
+    const long long grid = (total + 255) / 256;
+    if (grid > 2147483647ll) return fail(B2_ERR_SHAPE, "rows * n_kv_head * head_dim too large for one launch");
+    const dim3 g(static_cast<unsigned>(grid));
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a->dtype == B2_F16)
+        return a->head_dim == 64 ? launch_pdl(kv_q4_kernel<__half, 64, kAppend>, g, dim3(256), 0, s, p)
+                                 : launch_pdl(kv_q4_kernel<__half, 128, kAppend>, g, dim3(256), 0, s, p);
+    return a->head_dim == 64 ? launch_pdl(kv_q4_kernel<__nv_bfloat16, 64, kAppend>, g, dim3(256), 0, s, p)
+                             : launch_pdl(kv_q4_kernel<__nv_bfloat16, 128, kAppend>, g, dim3(256), 0, s, p);
+}
+
+int check_attn_q4_args(const B2PagedAttnQ4Args* a) {
+    if (a == nullptr) return fail(B2_ERR_NULL, "args is NULL");
+    if (a->dtype != B2_F16 && a->dtype != B2_BF16) return fail(B2_ERR_DTYPE, "q must be F16 or BF16");
+    if (a->out_dtype != B2_F32 && a->out_dtype != a->dtype)
+        return fail(B2_ERR_DTYPE, "out_dtype must be F32 or equal to dtype");
+    if (a->batch < 0) return fail(B2_ERR_SHAPE, "batch < 0");
+    const int rc = check_q4_shape(a->num_blocks, a->n_layer, a->n_kv_head, a->head_dim);
+    if (rc != B2_OK) return rc;
+    if (a->layer_idx < 0 || a->layer_idx >= a->n_layer) return fail(B2_ERR_SHAPE, "layer_idx out of range");
+    if (a->n_head <= 0 || a->n_head % a->n_kv_head != 0)
+        return fail(B2_ERR_SHAPE, "n_head must be a positive multiple of n_kv_head");
+    if (a->n_head / a->n_kv_head > kQ4MaxGroup) return fail(B2_ERR_UNSUPPORTED, "query-group size must be 1 to 8");
+    if (a->max_blocks_per_seq <= 0 || a->max_blocks_per_seq > (1 << 26) / B2_BLOCK_TOKENS)
+        return fail(B2_ERR_SHAPE, "max_blocks_per_seq out of range");
+    if (static_cast<double>(a->batch) * a->max_blocks_per_seq * a->n_kv_head >= 2147483648.0)
+        return fail(B2_ERR_SHAPE, "batch * max_blocks_per_seq * n_kv_head must stay below 2^31");
+    if (!(a->softcap >= 0.0f) || std::isinf(a->softcap)) return fail(B2_ERR_SHAPE, "softcap must be finite and >= 0");
+    if (!std::isfinite(a->scale)) return fail(B2_ERR_SHAPE, "scale must be finite");
+    if (a->window < 0) return fail(B2_ERR_SHAPE, "window < 0");
+    if (a->max_ctas < 0) return fail(B2_ERR_SHAPE, "max_ctas < 0");
+    if (a->batch == 0) return B2_OK;
+    if (!a->q || !a->kv_pool || !a->block_tables || !a->seq_lens || !a->out)
+        return fail(B2_ERR_NULL, "q, kv_pool, block_tables, seq_lens and out are required");
+    if (a->q_row_stride < static_cast<int64_t>(a->n_head) * a->head_dim)
+        return fail(B2_ERR_SHAPE, "q_row_stride < n_head*head_dim");
+    if (!aligned16(a->q) || !aligned16(a->kv_pool) || !aligned16(a->out) || a->q_row_stride % 8 != 0)
+        return fail(B2_ERR_ALIGN, "q, kv_pool and out must be 16-byte aligned, q_row_stride a multiple of 8");
+    return B2_OK;
+}
+
+template <typename T, typename OutT>
+int launch_attn_q4(const B2PagedAttnQ4Args* a, const Q4AttnParams& p, cudaStream_t s) {
+    const dim3 grid(static_cast<unsigned>(a->batch), static_cast<unsigned>(a->n_kv_head));
+    return a->head_dim == 64 ? launch_pdl(paged_decode_q4_kernel<T, OutT, 64>, grid, dim3(kQ4Threads), 0, s, p)
+                             : launch_pdl(paged_decode_q4_kernel<T, OutT, 128>, grid, dim3(kQ4Threads), 0, s, p);
+}
+
+}  // namespace
+}  // namespace b2
+
+extern "C" {
+
+int b2_block_map(const B2BlockMapArgs* a, b2_stream_t stream) {
+    using namespace b2;
+    if (a == nullptr) return fail(B2_ERR_NULL, "args is NULL");
+    if (a->n_seqs < 0 || a->max_rows < 0) return fail(B2_ERR_SHAPE, "n_seqs and max_rows must be >= 0");
+    if (a->n_seqs > B2_MAP_MAX_SEQS) return fail(B2_ERR_SHAPE, "n_seqs must be <= 16384");
+    if (a->max_blocks_per_seq <= 0 || a->max_blocks_per_seq > (1 << 26) / B2_BLOCK_TOKENS || a->num_blocks <= 0 ||
+        a->num_blocks > (1 << 27) - 1)
+        return fail(B2_ERR_SHAPE, "max_blocks_per_seq or num_blocks out of range");
+    if (a->max_rows > (1 << 30)) return fail(B2_ERR_SHAPE, "max_rows must be <= 2^30");
+    if (!a->free_count || !a->free_count_out) return fail(B2_ERR_NULL, "free_count and free_count_out are required");
+    if (a->n_seqs > 0 && (!a->seq_lens_pre || !a->free_list || !a->block_tables))
+        return fail(B2_ERR_NULL, "seq_lens_pre, free_list and block_tables are required");
+    if (a->max_rows > 0 && !a->slots) return fail(B2_ERR_NULL, "slots is required");
+    if (!aligned16(a->slots)) return fail(B2_ERR_ALIGN, "slots must be 16-byte aligned");
+    if (a->new_lens != nullptr && a->seq_lens_post == a->new_lens)
+        return fail(B2_ERR_SHAPE, "seq_lens_post must not alias new_lens");
+    BlockMapParams p{a->n_seqs, a->max_blocks_per_seq, a->num_blocks, a->max_rows, a->seq_lens_pre, a->new_lens,
+                     a->free_list, a->free_count, a->block_tables, a->slots, a->q_start, a->seq_lens_post,
+                     a->free_count_out};
+    static std::atomic<uint64_t> smem_set{0};
+    return launch_blocks(block_map_kernel, smem_set, 4 * (3 * a->n_seqs + 1), p, static_cast<cudaStream_t>(stream));
+}
+
+int b2_block_release(const B2BlockReleaseArgs* a, b2_stream_t stream) {
+    using namespace b2;
+    if (a == nullptr) return fail(B2_ERR_NULL, "args is NULL");
+    if (a->n_seqs < 0) return fail(B2_ERR_SHAPE, "n_seqs must be >= 0");
+    if (a->n_seqs > B2_MAP_MAX_SEQS) return fail(B2_ERR_SHAPE, "n_seqs must be <= 16384");
+    if (a->max_blocks_per_seq <= 0 || a->max_blocks_per_seq > (1 << 26) / B2_BLOCK_TOKENS || a->num_blocks <= 0 ||
+        a->num_blocks > (1 << 27) - 1)
+        return fail(B2_ERR_SHAPE, "max_blocks_per_seq or num_blocks out of range");
+    if (!a->free_count || !a->free_count_out) return fail(B2_ERR_NULL, "free_count and free_count_out are required");
+    if (a->n_seqs > 0 && (!a->block_tables || !a->seq_lens || !a->release || !a->free_list))
+        return fail(B2_ERR_NULL, "block_tables, seq_lens, release and free_list are required");
+    BlockReleaseParams p{a->n_seqs, a->max_blocks_per_seq, a->num_blocks, a->block_tables, a->seq_lens, a->release,
+                         a->free_list, a->free_count, a->free_count_out, a->seq_lens_out};
+    const int share = (a->n_seqs + kMapCluster - 1) / kMapCluster;
+    static std::atomic<uint64_t> smem_set{0};
+    return launch_blocks(block_release_kernel, smem_set, 4 * (2 * share + 1), p, static_cast<cudaStream_t>(stream));
+}
+
+size_t b2_kv_q4_pool_bytes(int32_t num_blocks, int32_t n_layer, int32_t n_kv_head, int32_t head_dim) {
+    using namespace b2;
+    if (check_q4_shape(num_blocks, n_layer, n_kv_head, head_dim) != B2_OK) return 0;
+    return static_cast<size_t>(num_blocks) * n_layer * n_kv_head * 20 * head_dim;
+}
+
+int b2_kv_append_q4(const B2KvQ4Args* a, b2_stream_t stream) { return b2::kv_q4<true>(a, stream); }
+
+int b2_kv_gather_q4(const B2KvQ4Args* a, b2_stream_t stream) { return b2::kv_q4<false>(a, stream); }
+
+size_t b2_paged_attention_q4_workspace_bytes(const B2PagedAttnQ4Args* a) {
+    using namespace b2;
+    if (check_attn_q4_args(a) != B2_OK) return 0;
+    return 256;
+}
+
+int b2_paged_attention_q4(const B2PagedAttnQ4Args* a, void* workspace, size_t workspace_bytes, b2_stream_t stream) {
+    using namespace b2;
+    const int rc = check_attn_q4_args(a);
+    if (rc != B2_OK || a->batch == 0) return rc;
+    const size_t need = b2_paged_attention_q4_workspace_bytes(a);
+    if (need == 0) return B2_ERR_DEVICE;
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need)
+        return fail(B2_ERR_WORKSPACE, "workspace NULL, not 16-byte aligned or smaller than b2_paged_attention_q4_workspace_bytes");
+    Q4AttnParams p;
+    p.q = a->q;
+    p.q_row_stride = a->q_row_stride;
+    p.pool = static_cast<const uint8_t*>(a->kv_pool);
+    p.block_tables = a->block_tables;
+    p.seq_lens = a->seq_lens;
+    p.key_starts = a->key_starts;
+    p.slopes = a->alibi_slopes;
+    p.out = a->out;
+    p.batch = a->batch;
+    p.n_head = a->n_head;
+    p.n_kv_head = a->n_kv_head;
+    p.group = a->n_head / a->n_kv_head;
+    p.mbps = a->max_blocks_per_seq;
+    p.layer_idx = a->layer_idx;
+    p.n_layer = a->n_layer;
+    p.num_blocks = a->num_blocks;
+    p.window = a->window;
+    p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
+    p.softcap = a->softcap;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a->out_dtype == B2_F32)
+        return a->dtype == B2_F16 ? launch_attn_q4<__half, float>(a, p, s) : launch_attn_q4<__nv_bfloat16, float>(a, p, s);
+    return a->dtype == B2_F16 ? launch_attn_q4<__half, __half>(a, p, s)
+                              : launch_attn_q4<__nv_bfloat16, __nv_bfloat16>(a, p, s);
+}
+
+}  // extern "C"
