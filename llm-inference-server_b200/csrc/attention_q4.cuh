@@ -1,9 +1,46 @@
 // attention_q4.cuh -- decode attention over the 4-bit paged pool (b2_paged_attention_q4).
 //
-// Plain form: one CTA per (sequence, kv head), a block of 16 tokens at a time
-// dequantised into shared memory, online softmax in fp32.
+// out[h] = sum_j p_j v_j / sum_j p_j,  p_j = 2^(x_j - R_h),  x_j the score in log2
+// units, k and v read as s (c - 8) + m per group of 32 dims.  One query token reads
+// every byte of its keys and values once, so the bound is HBM (1.25 head_dim
+// bytes per token and kv head) as long as turning codes into products stays
+// under the instruction rate that HBM leaves: about 3.5 instructions per
+// element and lane.  A multiply-add per element, query head and lane is over
+// that from two query heads per kv head on, so the products run on the tensor
+// cores (mma.sync: its operands come straight from the registers the codes are
+// unpacked in; tcgen05 would need them written back to shared memory at 4 times
+// their size first, more shared-memory traffic than the codes themselves).
+//
+//   * A 4-bit code masked into a 16-bit half IS an f16: bits 0-3 give c 2^-24,
+//     bits 4-7 give 16 c 2^-24 (subnormals; products with them are exact).  One
+//     AND makes two A-operand elements; no conversion, no bias.
+//   * Scores: A = 16 tokens x 16 dims of K codes, B = the query heads of the kv
+//     head (up to 8 columns).  Per group S += s (A q) + (m - 8 s) sum(q) in fp32.
+//     q is scaled by a power of two to at most 2^9, so its f16 form is exact
+//     down to 2^-23 of the row's largest element.
+//   * Values: A = V codes transposed (16 dims x 16 tokens), B = f16(p s 2^k) per
+//     group of 32 dims; C adds up sum p s c.  The f16 rounding of p s would count
+//     with c up to 15; adding the same product with A = -8 makes it count with
+//     c - 8 instead.  sum p m is a product with
+//     A = m.  Relative to an output of the values' spread that leaves ~2^-13 rms,
+//     under the rounding of an f16 output.  The k of 2^k keeps p s in f16's
+//     normal range whatever the values' size.
+//   * Softmax: R_h is a reference that moves only when a score passes it by 4
+//     (p <= 16); then, or when s 2^k grows past 2^11, the accumulators are
+//     rescaled.  Sums are fp32.
+//
+// Work: the (sequence, kv head, block) chunks of the call form one list,
+// split evenly over all warps (a multiple of chunks each, contiguous).  A warp
+// streams its chunks -- each one contiguous 20 * head_dim bytes -- through its own
+// ring of shared-memory stages with cp.async.bulk, without any CTA barrier.
+// Pieces of an item (sequence, kv head) that several warps hold meet in shared
+// memory, those of several CTAs in the workspace; the CTA that arrives last
+// merges them in CTA order, so results do not depend on timing.
 #pragma once
 
+#include <cfloat>
+
+#include "blocks.cuh"
 #include "kv_q4.cuh"
 
 namespace b2 {
@@ -17,9 +54,22 @@ struct Q4AttnParams {
     const int* key_starts;
     const float* slopes;
     void* out;
+    unsigned* ws_count;  // [grid]
+    float2* ws_ml;       // [2 grid][group]
+    float* ws_acc;       // [2 grid][group][head_dim]
     int batch, n_head, n_kv_head, group, mbps, layer_idx, n_layer, num_blocks, window;
+    int stages;
     float scale, softcap;
 };
+
+constexpr int kQ4Warps = 8;
+constexpr int kQ4Threads = 32 * kQ4Warps;
+constexpr int kQ4CtasPerSm = 2;
+constexpr int kQ4MaxGroup = 8;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Bytes of one piece's state in shared memory: [group][head_dim] sums, [group] (R, l).
+__host__ __device__ constexpr int q4_piece_bytes(int group, int dh) { return (group * (dh + 2) * 4 + 15) / 16 * 16; }
 
 // Visible keys of a sequence: [first, n).
 __device__ __forceinline__ void q4_range(const Q4AttnParams& p, int b, int* first, int* n, unsigned* err) {
@@ -35,89 +85,605 @@ __device__ __forceinline__ void q4_range(const Q4AttnParams& p, int b, int* firs
     *n = len;
 }
 
-constexpr int kQ4Threads = 256;
-constexpr int kQ4MaxGroup = 8;
+// Blocks that hold visible keys.
+__device__ __forceinline__ int q4_blocks(int first, int n) {
+    return first < n ? (n - 1) / kBlockTokens - first / kBlockTokens + 1 : 0;
+}
 
-template <typename T, typename OutT, int DH>
-__global__ void __launch_bounds__(kQ4Threads) paged_decode_q4_kernel(const Q4AttnParams p) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 half2_floats(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// G words from shared memory (G = 2 or 4).
+template <int G>
+__device__ __forceinline__ void ld_words(const uint8_t* p, uint32_t (&w)[G]) {
+    if constexpr (G == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    }
+}
+
+// One item's running state in a warp.  Lane = 4 r + i.
+template <int DH>
+struct Q4State {
+    static constexpr int G = DH / 32;
+    float acc[G][2][4];  // [group][dims 4r+0,1 | 4r+2,3][(dim, head 2i), (dim, 2i+1), (dim+1, 2i), (dim+1, 2i+1)]
+    float tz[4];         // row g: sum p m of group g
+    float ref[2], l[2];  // heads 2i, 2i+1; l is this lane's share
+    int k;
+    uint32_t s_limit;    // param words from here on need a smaller k
+    uint32_t qf[G][4];   // B fragments of head r
+    float qs[G][2];      // 2^-24 sum of q over the group, heads 2i, 2i+1
+    float sc[2];         // S -> score (log2 units; with a cap: the exponent's argument)
+    float slope[2];      // log2 units
+};
+
+__device__ __forceinline__ uint32_t q4_s_limit(int k) {
+    return static_cast<uint32_t>(min((26 - k) << 10, 0xffff)) << 16;  // words with s >= 2^(11 - k)
+}
+
+// Loads the query heads of item (b, hk) and clears the sums.
+template <typename T, int DH>
+__device__ __forceinline__ void q4_start(const Q4AttnParams& p, int b, int hk, Q4State<DH>& st) {
+    constexpr int G = DH / 32;
+    const int lane = threadIdx.x & 31, r = lane >> 2, i = lane & 3;
+    float x[G][8];
+    float top = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (r < p.group)
+            raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_row_stride +
+                                                       static_cast<long long>(hk * p.group + r) * DH + g * 32 + i * 8));
+        unpack16<T>(raw, x[g]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[g][e]));
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    // 2^(8 - floor(log2 top)): the largest |q| lands in [2^8, 2^9)
+    const int e2 = static_cast<int>(__float_as_uint(top) >> 23);  // biased exponent, 255 for an infinity
+    const int up = e2 == 255 ? 0 : min(135 - e2, 126);
+    const float norm = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+    float qsum[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const float f16th = norm * 0.0625f;
+        st.qf[g][0] = half2_bits(x[g][0] * norm, x[g][4] * norm);
+        st.qf[g][1] = half2_bits(x[g][1] * f16th, x[g][5] * f16th);
+        st.qf[g][2] = half2_bits(x[g][2] * norm, x[g][6] * norm);
+        st.qf[g][3] = half2_bits(x[g][3] * f16th, x[g][7] * f16th);
+        const float2 a = half2_floats(st.qf[g][0]), c = half2_floats(st.qf[g][1]);
+        const float2 d = half2_floats(st.qf[g][2]), f = half2_floats(st.qf[g][3]);
+        float sum = (a.x + a.y) + (d.x + d.y) + 16.0f * ((c.x + c.y) + (f.x + f.y));
+#pragma unroll
+        for (int s = 1; s < 4; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        qsum[g] = sum * 0x1p-24f;
+    }
+    // score = S 2^24 / norm * scale; the cap's argument is 2 score / cap (exp of it in log2 units)
+    const float unit = p.softcap > 0.0f ? 2.0f * kLog2e * p.scale / p.softcap : kLog2e * p.scale;
+    const float sc = unit * 0x1p24f * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int src = 4 * (2 * i + h);
+#pragma unroll
+        for (int g = 0; g < G; ++g) st.qs[g][h] = __shfl_sync(0xffffffffu, qsum[g], src);
+        st.sc[h] = __shfl_sync(0xffffffffu, sc, src);
+        st.slope[h] = p.slopes != nullptr && 2 * i + h < p.group ? __ldg(p.slopes + hk * p.group + 2 * i + h) * kLog2e : 0.0f;
+        st.ref[h] = -FLT_MAX;
+        st.l[h] = 0.0f;
+    }
+    st.k = 18;
+    st.s_limit = q4_s_limit(18);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        st.tz[c] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) st.acc[g][0][c] = st.acc[g][1][c] = 0.0f;
+    }
+}
+
+// One chunk of 16 tokens, positions blk * 16 on, keys [first, n) visible.
+template <int DH>
+__device__ __forceinline__ void q4_chunk(const Q4AttnParams& p, uint8_t* stage, int blk, int first, int n,
+                                         Q4State<DH>& st) {
     using C = Q4Chunk<DH>;
-    __shared__ float s_q[kQ4MaxGroup][DH], s_k[kBlockTokens][DH + 1], s_v[kBlockTokens][DH];
-    __shared__ float s_x[kQ4MaxGroup][kBlockTokens];
+    constexpr int G = DH / 32;
+    constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
+    const int lane = threadIdx.x & 31, r = lane >> 2, i = lane & 3;
+    // Token of product row r (and r + 8: 8 later).  Chosen so that the rows' K words,
+    // the lanes' V words and all params are read without bank conflicts.
+    const int tk = (r & 1) ? 4 + ((r >> 1) ^ 3) : r >> 1;
+    const int ta = i, tb = 4 + (i ^ 3);  // V: product columns 2i and 2i + 1
+    const bool edge = blk * kBlockTokens < first || blk * kBlockTokens + kBlockTokens > n;
+    if (edge) {
+        // What masked tokens hold may be anything, NaN included: 0 * NaN must not reach the sums.
+        if (lane < kBlockTokens) {
+            const int j = blk * kBlockTokens + lane;
+            if (j < first || j >= n) {
+#pragma unroll
+                for (int g = 0; g < G; ++g) *reinterpret_cast<uint32_t*>(stage + C::kVParams + C::param(lane, g)) = 0;
+            }
+        }
+        // these generic writes come before the copy that refills the stage
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+    }
+    float x[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};  // [token tk, tk + 8][head 2i, 2i + 1]
+    {
+        uint32_t ka[G], kb[G], pa[G], pb[G];
+        ld_words<G>(stage + C::k_word(tk, i, 0), ka);
+        ld_words<G>(stage + C::k_word(tk + 8, i, 0), kb);
+        ld_words<G>(stage + C::kKParams + C::param(tk, 0), pa);
+        ld_words<G>(stage + C::kKParams + C::param(tk + 8, 0), pb);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma_f16(c, ka[g] & kLow, kb[g] & kLow, ka[g] & kHigh, kb[g] & kHigh, st.qf[g][0], st.qf[g][1]);
+            const uint32_t ua = ka[g] >> 8, ub = kb[g] >> 8;
+            mma_f16(c, ua & kLow, ub & kLow, ua & kHigh, ub & kHigh, st.qf[g][2], st.qf[g][3]);
+            const float2 a = half2_floats(pa[g]), b = half2_floats(pb[g]);  // (m, s)
+            const float ma = fmaf(-8.0f, a.y, a.x), mb = fmaf(-8.0f, b.y, b.x);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                x[0][h] = fmaf(a.y, c[h], fmaf(ma, st.qs[g][h], x[0][h]));
+                x[1][h] = fmaf(b.y, c[2 + h], fmaf(mb, st.qs[g][h], x[1][h]));
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x[t][h] *= st.sc[h];
+    if (p.softcap > 0.0f) {
+        const float cap = p.softcap * kLog2e;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)  // tanh(y) = 1 - 2 / (1 + e^2y): 2^-23 absolute, to be multiplied by the cap
+                x[t][h] = cap - __fdividef(2.0f * cap, 1.0f + ex2_approx(x[t][h]));
+    }
+    if (p.slopes != nullptr) {
+        const float d = static_cast<float>(blk * kBlockTokens + tk - (n - 1));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            x[0][h] = fmaf(st.slope[h], d, x[0][h]);
+            x[1][h] = fmaf(st.slope[h], d + 8.0f, x[1][h]);
+        }
+    }
+    if (edge) {
+        const int j = blk * kBlockTokens + tk;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (j < first || j >= n) x[0][h] = -INFINITY;
+            if (j + 8 < first || j + 8 >= n) x[1][h] = -INFINITY;
+        }
+    }
+    uint32_t va[G], vb[G];  // V params of tokens tk, tk + 8
+    ld_words<G>(stage + C::kVParams + C::param(tk, 0), va);
+    ld_words<G>(stage + C::kVParams + C::param(tk + 8, 0), vb);
+    float top[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) top[h] = fmaxf(x[0][h], x[1][h]);
+    uint32_t s_top = 0;
+#pragma unroll
+    for (int g = 0; g < G; ++g) s_top = max(s_top, max(va[g], vb[g]));
+    if (__any_sync(0xffffffffu, top[0] - 4.0f > st.ref[0] || top[1] - 4.0f > st.ref[1] || s_top >= st.s_limit)) {
+        s_top = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {  // NaN and infinite steps do not count
+            if (va[g] < 0x7c000000u) s_top = max(s_top, va[g]);
+            if (vb[g] < 0x7c000000u) s_top = max(s_top, vb[g]);
+        }
+        s_top = __reduce_max_sync(0xffffffffu, s_top);
+        const int k = min(st.k, 18 - static_cast<int>(s_top >> 26));  // s 2^k < 2^4
+        const float by = __uint_as_float(static_cast<uint32_t>(127 + k - st.k) << 23);
+        st.k = k;
+        st.s_limit = q4_s_limit(k);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
+            const float ref = fmaxf(st.ref[h], top[h]);
+            const float f = ex2_approx(st.ref[h] - ref);
+            st.ref[h] = ref;
+            st.l[h] *= f;
+            st.tz[h] *= f;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    st.acc[g][t][h] *= f * by;
+                    st.acc[g][t][2 + h] *= f * by;
+                }
+        }
+    }
+    float w[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        w[0][h] = ex2_approx(x[0][h] - st.ref[h]);
+        w[1][h] = ex2_approx(x[1][h] - st.ref[h]);
+        st.l[h] += w[0][h] + w[1][h];
+    }
+    {  // sum p m: A rows = groups (rows from G on repeat them, unused)
+        const uint8_t* pm = stage + C::kVParams + (r & (G - 1)) * 4;
+        const uint32_t m0 = *reinterpret_cast<const uint32_t*>(pm + C::param(ta, 0));
+        const uint32_t m1 = *reinterpret_cast<const uint32_t*>(pm + C::param(tb, 0));
+        const uint32_t m2 = *reinterpret_cast<const uint32_t*>(pm + C::param(ta + 8, 0));
+        const uint32_t m3 = *reinterpret_cast<const uint32_t*>(pm + C::param(tb + 8, 0));
+        const uint32_t b0 = transpose8x8(half2_bits(w[0][0], w[0][1]));
+        const uint32_t b1 = transpose8x8(half2_bits(w[1][0], w[1][1]));
+        mma_f16(st.tz, __byte_perm(m0, m1, 0x5410), 0, __byte_perm(m2, m3, 0x5410), 0, b0, b1);
+    }
+    const float up = __uint_as_float(static_cast<uint32_t>(127 + st.k) << 23);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[t][h] *= up;
+    uint32_t v[4][G / 2];  // words of tokens ta, tb, ta + 8, tb + 8: groups 2w (low) and 2w + 1 (high)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const uint8_t* at = stage + C::v_unit((t & 1 ? tb : ta) + (t & 2 ? 8 : 0), r, 0);
+        if constexpr (G == 4) {
+            const uint2 u = *reinterpret_cast<const uint2*>(at);
+            v[t][0] = u.x, v[t][1] = u.y;
+        } else {
+            v[t][0] = *reinterpret_cast<const uint32_t*>(at);
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        const float sa = half2_floats(va[g]).y, sb = half2_floats(vb[g]).y;
+        const uint32_t b0 = transpose8x8(half2_bits(w[0][0] * sa, w[0][1] * sa));
+        const uint32_t b1 = transpose8x8(half2_bits(w[1][0] * sb, w[1][1] * sb));
+        const uint32_t pick = g & 1 ? 0x7632 : 0x5410;
+        const uint32_t u0 = __byte_perm(v[0][g / 2], v[1][g / 2], pick), u1 = __byte_perm(v[2][g / 2], v[3][g / 2], pick);
+        mma_f16(st.acc[g][0], u0 & kLow, u0 & kHigh, u1 & kLow, u1 & kHigh, b0, b1);
+        const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
+        mma_f16(st.acc[g][1], w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh, b0, b1);
+        // -8 in the units of even and odd dims: -8 2^-24 and -8 16 2^-24
+        mma_f16(st.acc[g][0], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
+        mma_f16(st.acc[g][1], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
+    }
+}
+
+// Ends an item: this lane's sums for heads 2i + h, dims 32 g + 4 r .. + 3, and l over all tokens.
+template <int DH>
+__device__ __forceinline__ void q4_finish(Q4State<DH>& st, float (&out)[2][DH / 32][4], float (&l)[2]) {
+    constexpr int G = DH / 32;
+    const int i = threadIdx.x & 3;
+    const float f = __uint_as_float(static_cast<uint32_t>(127 + 24 - st.k) << 23);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] = st.l[h];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], d);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float c = __shfl_sync(0xffffffffu, st.tz[h], 4 * g + i);
+            out[h][g][0] = fmaf(st.acc[g][0][h], f, c);
+            out[h][g][1] = fmaf(st.acc[g][0][2 + h], f * 0.0625f, c);
+            out[h][g][2] = fmaf(st.acc[g][1][h], f, c);
+            out[h][g][3] = fmaf(st.acc[g][1][2 + h], f * 0.0625f, c);
+        }
+    }
+}
+
+template <typename OutT>
+__device__ __forceinline__ void q4_store4(OutT* at, float a, float b, float c, float d) {
+    if constexpr (sizeof(OutT) == 4) {
+        *reinterpret_cast<float4*>(at) = make_float4(a, b, c, d);
+    } else {
+        OutT t[4] = {Elem<OutT>::from_f(a), Elem<OutT>::from_f(b), Elem<OutT>::from_f(c), Elem<OutT>::from_f(d)};
+        *reinterpret_cast<uint2*>(at) = *reinterpret_cast<const uint2*>(t);
+    }
+}
+
+struct Q4Entry {
+    int item;        // -1: none
+    unsigned start;  // the item's first chunk in the list
+    unsigned count;  // its chunks
+};
+
+// Dynamic shared memory: [warp][stages] chunks, [warp] first pieces, [warp][stages] barriers.
+template <typename T, typename OutT, int DH>
+__global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kernel(const Q4AttnParams p) {
+    using C = Q4Chunk<DH>;
+    constexpr int G = DH / 32;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ unsigned s_seg[kQ4Threads + 1], s_scan[33];
+    __shared__ Q4Entry s_entry[2 * kQ4Warps];
+    __shared__ Q4Entry s_open[2];  // items of this CTA that other CTAs hold parts of
+    __shared__ int s_last[2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane & 3, r = lane >> 2;
+    const int piece_bytes = q4_piece_bytes(p.group, DH);
+    uint8_t* ring = smem + static_cast<size_t>(warp) * p.stages * C::kBytes;
+    uint8_t* pieces = smem + static_cast<size_t>(kQ4Warps) * p.stages * C::kBytes;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(pieces + kQ4Warps * piece_bytes) + warp * p.stages;
+    // A piece's state: slot 0 (the warp's first chunks) has its own room, slot 1 (its last) takes the drained ring.
+    auto piece_at = [&](int w, int slot) {
+        return reinterpret_cast<float*>(slot == 0 ? pieces + w * piece_bytes
+                                                  : smem + static_cast<size_t>(w) * p.stages * C::kBytes);
+    };
+    if (lane == 0) {
+        for (int s = 0; s < p.stages; ++s) mbar_init(bars + s, 1);
+        fence_mbar_init();
+    }
+    if (tid < 2 * kQ4Warps) s_entry[tid].item = -1;
+    if (tid < 2) s_open[tid].item = -1;
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.x, hk = blockIdx.y, tid = threadIdx.x;
+
+    // The list: chunks before each thread's share of the sequences.
     unsigned err = 0;
-    int first, n;
-    q4_range(p, b, &first, &n, &err);
-    for (int e = tid; e < p.group * DH; e += kQ4Threads) {
-        const int h = hk * p.group + e / DH;
-        s_q[e / DH][e % DH] =
-            Elem<T>::to_f(static_cast<const T*>(p.q)[b * p.q_row_stride + static_cast<long long>(h) * DH + e % DH]);
+    const int per = (p.batch + kQ4Threads - 1) / kQ4Threads;
+    unsigned mine = 0;
+    for (int b = min(tid * per, p.batch); b < min((tid + 1) * per, p.batch); ++b) {
+        int first, n;
+        q4_range(p, b, &first, &n, &err);
+        mine += static_cast<unsigned>(q4_blocks(first, n)) * p.n_kv_head;
     }
-    constexpr int kOwn = kQ4MaxGroup * DH / kQ4Threads;
-    float m[kOwn], l[kOwn], acc[kOwn];
-#pragma unroll
-    for (int o = 0; o < kOwn; ++o) {
-        m[o] = -INFINITY;
-        l[o] = acc[o] = 0.0f;
-    }
-    for (int blk = first / kBlockTokens; blk * kBlockTokens < n; ++blk) {
-        int id = __ldg(p.block_tables + static_cast<size_t>(b) * p.mbps + blk);
+    if (blockIdx.x != 0) err = 0;
+    unsigned total;
+    s_seg[tid] = block_scan(mine, 0x7fffffffu, s_scan, &total);
+    __syncthreads();
+    // Fewer CTAs than launched where a warp would get less than a chunk.
+    const unsigned ctas = max(1u, min(gridDim.x, (total + kQ4Warps - 1) / kQ4Warps));
+    const unsigned long long parts = static_cast<unsigned long long>(ctas) * kQ4Warps;
+    auto bound = [&](unsigned part) { return static_cast<unsigned>(static_cast<unsigned long long>(total) * part / parts); };
+    const bool active = blockIdx.x < ctas;
+    const unsigned c0 = active ? bound(blockIdx.x * kQ4Warps + warp) : 0;
+    const unsigned c1 = active ? bound(blockIdx.x * kQ4Warps + warp + 1) : 0;
+
+    // Lane's chunk of the 32 from `from` on: where it lies and what it is.
+    auto locate = [&](unsigned from, unsigned* chunk, int* item, int* blk) {
+        const unsigned c = from + lane;
+        *chunk = 0;
+        *item = -1;
+        *blk = 0;
+        if (c >= c1) return;
+        const int seg = last_at_most(s_seg, kQ4Threads, c);
+        unsigned base = s_seg[seg];
+        int b = seg * per, first, n, nb;
+        unsigned none = 0;
+        for (;; ++b) {
+            q4_range(p, b, &first, &n, &none);
+            nb = q4_blocks(first, n);
+            if (c < base + static_cast<unsigned>(nb) * p.n_kv_head || b + 1 == p.batch) break;
+            base += static_cast<unsigned>(nb) * p.n_kv_head;
+        }
+        const int h = static_cast<int>(c - base) / nb;
+        *blk = first / kBlockTokens + static_cast<int>(c - base) - h * nb;
+        *item = b * p.n_kv_head + h;
+        int id = __ldg(p.block_tables + static_cast<size_t>(b) * p.mbps + *blk);
         if (id < 0 || id >= p.num_blocks) {
             err |= B2_DEVERR_BLOCK_ID;
             id = min(max(id, 0), p.num_blocks - 1);
         }
-        const uint8_t* chunk = p.pool + ((static_cast<size_t>(id) * p.n_layer + p.layer_idx) * p.n_kv_head + hk) *
-                                            static_cast<size_t>(C::kBytes);
-        __syncthreads();
-        for (int e = tid; e < kBlockTokens * DH; e += kQ4Threads) {
-            const int t = e / DH, d = e % DH, g = d / 32, in = d % 32;
-            const uint32_t kw = *reinterpret_cast<const uint32_t*>(chunk + C::k_word(t, in / 8, g));
-            const uint32_t vw = *reinterpret_cast<const uint16_t*>(chunk + C::v_unit(t, in / 4, g));
-            const __half2 kp = *reinterpret_cast<const __half2*>(chunk + C::kKParams + C::param(t, g));
-            const __half2 vp = *reinterpret_cast<const __half2*>(chunk + C::kVParams + C::param(t, g));
-            const int j = blk * kBlockTokens + t;
-            s_k[t][d] = fmaf(static_cast<float>(static_cast<int>(kw >> (4 * (in % 8)) & 15u) - 8), __high2float(kp), __low2float(kp));
-            s_v[t][d] = j < first || j >= n ? 0.0f
-                                            : fmaf(static_cast<float>(static_cast<int>(vw >> (4 * (in % 4)) & 15u) - 8),
-                                                   __high2float(vp), __low2float(vp));
+        *chunk = static_cast<unsigned>((static_cast<long long>(id) * p.n_layer + p.layer_idx) * p.n_kv_head + h);
+    };
+    unsigned new_chunk = 0, old_chunk = 0;
+    int new_item = -1, new_blk = 0, old_item = -1, old_blk = 0;
+    unsigned issued = c0, window_at = c0;  // next chunk to copy; first chunk of the new window of 32
+    auto issue = [&](int stage) {  // all lanes; copies chunk `issued`
+        if (issued == window_at + 32) {
+            old_chunk = new_chunk, old_item = new_item, old_blk = new_blk;
+            window_at = issued;
+            locate(issued, &new_chunk, &new_item, &new_blk);
         }
-        __syncthreads();
-        if (tid < p.group * kBlockTokens) {
-            const int h = tid / kBlockTokens, t = tid % kBlockTokens, j = blk * kBlockTokens + t;
-            float x = 0.0f;
-            for (int d = 0; d < DH; ++d) x = fmaf(s_q[h][d], s_k[t][d], x);
-            x *= p.scale;
-            if (p.softcap > 0.0f) x = p.softcap * tanhf(x / p.softcap);
-            if (p.slopes != nullptr) x = fmaf(__ldg(p.slopes + hk * p.group + h), static_cast<float>(j - (n - 1)), x);
-            s_x[h][t] = j < first || j >= n ? -INFINITY : x;
+        const unsigned chunk = __shfl_sync(0xffffffffu, new_chunk, issued - window_at);
+        if (lane == 0) {
+            mbar_arrive_expect_tx(bars + stage, C::kBytes);
+            bulk_g2s(ring + stage * C::kBytes, p.pool + static_cast<size_t>(chunk) * C::kBytes, C::kBytes, bars + stage);
         }
-        __syncthreads();
+        ++issued;
+    };
+    if (c0 < c1) {
+        locate(c0, &new_chunk, &new_item, &new_blk);
+        for (int s = 0; s < p.stages && issued < c1; ++s) issue(s);
+    }
+
+    Q4State<DH> st;
+    int item = -1, first = 0, n = 0, from_blk = 0;
+    unsigned from = c0;
+    // Writes the item's result, or this warp's part of it where it holds not all of its chunks.
+    auto end_item = [&](unsigned upto) {
+        float o[2][G][4], l[2];
+        q4_finish<DH>(st, o, l);
+        const int b = item / p.n_kv_head, hk = item - b * p.n_kv_head;
+        const int nb = q4_blocks(first, n);
+        if (upto - from == static_cast<unsigned>(nb)) {
 #pragma unroll
-        for (int o = 0; o < kOwn; ++o) {
-            const int e = tid + o * kQ4Threads, h = e / DH, d = e % DH;
-            if (h >= p.group) continue;
-            float mn = m[o];
-            for (int t = 0; t < kBlockTokens; ++t) mn = fmaxf(mn, s_x[h][t]);
-            const float c = expf(m[o] - mn);
-            l[o] *= c;
-            acc[o] *= c;
-            for (int t = 0; t < kBlockTokens; ++t) {
-                const float w = expf(s_x[h][t] - mn);
-                l[o] += w;
-                acc[o] = fmaf(w, s_v[t][d], acc[o]);
+            for (int h = 0; h < 2; ++h)
+                if (2 * i + h < p.group) {
+                    const float inv = 1.0f / l[h];
+                    OutT* row = static_cast<OutT*>(p.out) +
+                                (static_cast<size_t>(b) * p.n_head + hk * p.group + 2 * i + h) * DH + 4 * r;
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+                        q4_store4<OutT>(row + 32 * g, o[h][g][0] * inv, o[h][g][1] * inv, o[h][g][2] * inv, o[h][g][3] * inv);
+                }
+            return;
+        }
+        const int slot = upto == c1 ? 1 : 0;
+        float* at = piece_at(warp, slot);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (2 * i + h < p.group) {
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+                    *reinterpret_cast<float4*>(at + (2 * i + h) * DH + 32 * g + 4 * r) =
+                        make_float4(o[h][g][0], o[h][g][1], o[h][g][2], o[h][g][3]);
+                if (r == 0) *reinterpret_cast<float2*>(at + p.group * DH + 2 * (2 * i + h)) = make_float2(st.ref[h], l[h]);
             }
-            m[o] = mn;
+        if (lane == 0)
+            s_entry[2 * warp + slot] = Q4Entry{item, from - static_cast<unsigned>(from_blk - first / kBlockTokens),
+                                               static_cast<unsigned>(nb)};
+    };
+    int stage = 0;
+    uint32_t parity = 0;
+    bool alive = true;
+    unsigned c = c0;
+    for (; c < c1; ++c) {
+        const bool in_new = c >= window_at;
+        const int src = static_cast<int>(in_new ? c - window_at : c - (window_at - 32));
+        const int it = __shfl_sync(0xffffffffu, in_new ? new_item : old_item, src);
+        const int blk = __shfl_sync(0xffffffffu, in_new ? new_blk : old_blk, src);
+        if (it != item) {
+            if (item >= 0) end_item(c);
+            item = it;
+            from = c;
+            from_blk = blk;
+            const int b = it / p.n_kv_head;
+            unsigned none = 0;
+            q4_range(p, b, &first, &n, &none);
+            q4_start<T, DH>(p, b, it - b * p.n_kv_head, st);
+        }
+        alive = __all_sync(0xffffffffu, mbar_wait_bounded(bars + stage, parity));
+        if (!alive) break;
+        q4_chunk<DH>(p, ring + stage * C::kBytes, blk, first, n, st);
+        __syncwarp();  // every lane is done with the stage
+        if (issued < c1) issue(stage);
+        if (++stage == p.stages) {
+            stage = 0;
+            parity ^= 1;
         }
     }
-#pragma unroll
-    for (int o = 0; o < kOwn; ++o) {
-        const int e = tid + o * kQ4Threads, h = e / DH, d = e % DH;
-        if (h >= p.group) continue;
-        static_cast<OutT*>(p.out)[(static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH + d] =
-            Elem<OutT>::from_f(first < n ? acc[o] / l[o] : 0.0f);
+    if (alive) {
+        if (item >= 0) end_item(c1);
+    } else {  // the copies in flight end before this CTA's shared memory goes
+        err |= B2_DEVERR_TIMEOUT;
+        for (; c < issued; ++c) {
+            mbar_wait_bounded(bars + stage, parity);
+            if (++stage == p.stages) {
+                stage = 0;
+                parity ^= 1;
+            }
+        }
     }
-    if (err != 0 && tid == 0 && hk == 0) flag_error(err);
+    __syncthreads();
+
+    // Pieces of one item lie in consecutive entries; the warp that holds the first of them merges them.
+    const unsigned cta0 = active ? bound(blockIdx.x * kQ4Warps) : 0, cta1 = active ? bound((blockIdx.x + 1) * kQ4Warps) : 0;
+    for (int slot = 0; slot < 2; ++slot) {
+        const int e0 = 2 * warp + slot;
+        const Q4Entry en = s_entry[e0];
+        if (en.item < 0) continue;
+        int prev = e0 - 1;
+        while (prev >= 0 && s_entry[prev].item < 0) --prev;
+        if (prev >= 0 && s_entry[prev].item == en.item) continue;
+        const bool whole = en.start >= cta0 && en.start + en.count <= cta1;
+        const int open = en.start >= cta0 ? 1 : 0;
+        const size_t at = static_cast<size_t>(blockIdx.x) * 2 + open;
+        const int b = en.item / p.n_kv_head, hk = en.item - b * p.n_kv_head;
+        for (int h = 0; h < p.group; ++h) {
+            float top = -FLT_MAX;
+            for (int e = e0; e < 2 * kQ4Warps; ++e)
+                if (s_entry[e].item == en.item) top = fmaxf(top, piece_at(e >> 1, e & 1)[p.group * DH + 2 * h]);
+            float l = 0.0f;
+            float sum[G];
+#pragma unroll
+            for (int g = 0; g < G; ++g) sum[g] = 0.0f;
+            for (int e = e0; e < 2 * kQ4Warps; ++e)
+                if (s_entry[e].item == en.item) {
+                    const float* pc = piece_at(e >> 1, e & 1);
+                    const float f = ex2_approx(pc[p.group * DH + 2 * h] - top);
+                    l = fmaf(pc[p.group * DH + 2 * h + 1], f, l);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) sum[g] = fmaf(pc[h * DH + 32 * g + lane], f, sum[g]);
+                }
+            if (whole) {
+                const float inv = 1.0f / l;
+                OutT* row = static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH;
+#pragma unroll
+                for (int g = 0; g < G; ++g) row[32 * g + lane] = Elem<OutT>::from_f(sum[g] * inv);
+            } else {
+#pragma unroll
+                for (int g = 0; g < G; ++g) __stcg(p.ws_acc + (at * p.group + h) * DH + 32 * g + lane, sum[g]);
+                if (lane == 0) __stcg(p.ws_ml + at * p.group + h, make_float2(top, l));
+            }
+        }
+        if (!whole && lane == 0) s_open[open] = en;
+    }
+    __syncthreads();
+
+    // Items over several CTAs: the last CTA to arrive merges, in CTA order.
+    auto cta_of = [&](unsigned chunk) {
+        return static_cast<unsigned>(((chunk + 1ull) * ctas - 1) / total);
+    };
+    if (tid < 2) {
+        s_last[tid] = 0;
+        if (s_open[tid].item >= 0) {
+            const unsigned f = cta_of(s_open[tid].start), last = cta_of(s_open[tid].start + s_open[tid].count - 1);
+            __threadfence();
+            const unsigned before = atomicAdd(p.ws_count + f, 1u);
+            if (before == last - f) {
+                s_last[tid] = 1;
+                p.ws_count[f] = 0;
+                __threadfence();
+            }
+        }
+    }
+    __syncthreads();
+    for (int open = 0; open < 2; ++open) {
+        if (!s_last[open]) continue;
+        const Q4Entry en = s_open[open];
+        const unsigned f = cta_of(en.start), last = cta_of(en.start + en.count - 1);
+        const int b = en.item / p.n_kv_head, hk = en.item - b * p.n_kv_head;
+        for (int e = tid * 4; e < p.group * DH; e += kQ4Threads * 4) {
+            const int h = e / DH, d = e % DH;
+            float top = -FLT_MAX, l = 0.0f;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (unsigned j = f; j <= last; ++j)
+                top = fmaxf(top, __ldcg(p.ws_ml + (2ull * j + (j == f ? 1 : 0)) * p.group + h).x);
+#pragma unroll 4
+            for (unsigned j = f; j <= last; ++j) {
+                const size_t at = (2ull * j + (j == f ? 1 : 0)) * p.group + h;
+                const float2 ml = __ldcg(p.ws_ml + at);
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + at * DH + d));
+                const float w = ex2_approx(ml.x - top);
+                l = fmaf(ml.y, w, l);
+                sum.x = fmaf(v.x, w, sum.x);
+                sum.y = fmaf(v.y, w, sum.y);
+                sum.z = fmaf(v.z, w, sum.z);
+                sum.w = fmaf(v.w, w, sum.w);
+            }
+            const float inv = 1.0f / l;
+            q4_store4<OutT>(static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH + d,
+                            sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+        }
+    }
+    // Sequences without a visible key.
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        int lo, len;
+        unsigned none = 0;
+        q4_range(p, b, &lo, &len, &none);
+        if (lo < len) continue;
+        OutT* row = static_cast<OutT*>(p.out) + static_cast<size_t>(b) * p.n_head * DH;
+        for (int e = tid * 4; e < p.n_head * DH; e += kQ4Threads * 4) q4_store4<OutT>(row + e, 0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    if (err != 0) flag_error(err);
 }
 
 }  // namespace b2

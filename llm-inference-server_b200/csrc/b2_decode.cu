@@ -1651,11 +1651,48 @@ int check_attn_q4_args(const B2PagedAttnQ4Args* a) {
     return B2_OK;
 }
 
+struct Q4Plan {
+    int grid = 0, stages = 0, smem = 0;
+    size_t ws_count = 0, ws_ml = 0, ws_total = 0;  // [counters][(R, l)][sums]
+};
+
+// Two CTAs per SM; as many ring stages (up to 8) as their half of the shared memory holds.
+int plan_attn_q4(const B2PagedAttnQ4Args* a, Q4Plan* pl) {
+    int dev = -1;
+    const DeviceInfo di = device_info(&dev);
+    if (dev < 0 || di.sms <= 0) return fail(B2_ERR_DEVICE, "no current CUDA device");
+    const int group = a->n_head / a->n_kv_head;
+    const int pieces = kQ4Warps * q4_piece_bytes(group, a->head_dim);
+    const int per_stage = kQ4Warps * (20 * a->head_dim + 8);
+    const int room = di.smem_per_sm / kQ4CtasPerSm - 1024 - 2048;  // reserved and static shared memory
+    pl->stages = std::min(8, (room - pieces) / per_stage);
+    // a warp's last piece is kept in its drained ring
+    if (pl->stages < 2 || pl->stages * 20 * a->head_dim < q4_piece_bytes(group, a->head_dim))
+        return fail(B2_ERR_UNSUPPORTED, "4-bit attention: shared memory");
+    pl->smem = pieces + pl->stages * per_stage;
+    pl->grid = di.sms * kQ4CtasPerSm;
+    if (a->max_ctas > 0) pl->grid = std::min(pl->grid, a->max_ctas);
+    const size_t slots = 2 * static_cast<size_t>(pl->grid) * group;
+    pl->ws_count = align_up(static_cast<size_t>(pl->grid) * sizeof(unsigned), 256);
+    pl->ws_ml = align_up(slots * sizeof(float2), 256);
+    pl->ws_total = pl->ws_count + pl->ws_ml + align_up(slots * a->head_dim * sizeof(float), 256);
+    return B2_OK;
+}
+
+template <typename T, typename OutT, int DH>
+int launch_attn_q4_t(const Q4Plan& pl, const Q4AttnParams& p, cudaStream_t s) {
+    auto kern = paged_decode_q4_kernel<T, OutT, DH>;
+    static std::atomic<uint64_t> smem_set{0};
+    int dev = -1;
+    const DeviceInfo di = device_info(&dev);
+    const int rc = ensure_max_smem(kern, smem_set, dev, di.smem_per_sm / kQ4CtasPerSm - 1024 - 2048);
+    if (rc != B2_OK) return rc;
+    return launch_pdl(kern, dim3(static_cast<unsigned>(pl.grid)), dim3(kQ4Threads), pl.smem, s, p);
+}
+
 template <typename T, typename OutT>
-int launch_attn_q4(const B2PagedAttnQ4Args* a, const Q4AttnParams& p, cudaStream_t s) {
-    const dim3 grid(static_cast<unsigned>(a->batch), static_cast<unsigned>(a->n_kv_head));
-    return a->head_dim == 64 ? launch_pdl(paged_decode_q4_kernel<T, OutT, 64>, grid, dim3(kQ4Threads), 0, s, p)
-                             : launch_pdl(paged_decode_q4_kernel<T, OutT, 128>, grid, dim3(kQ4Threads), 0, s, p);
+int launch_attn_q4(const B2PagedAttnQ4Args* a, const Q4Plan& pl, const Q4AttnParams& p, cudaStream_t s) {
+    return a->head_dim == 64 ? launch_attn_q4_t<T, OutT, 64>(pl, p, s) : launch_attn_q4_t<T, OutT, 128>(pl, p, s);
 }
 
 }  // namespace
@@ -1716,17 +1753,19 @@ int b2_kv_gather_q4(const B2KvQ4Args* a, b2_stream_t stream) { return b2::kv_q4<
 
 size_t b2_paged_attention_q4_workspace_bytes(const B2PagedAttnQ4Args* a) {
     using namespace b2;
-    if (check_attn_q4_args(a) != B2_OK) return 0;
-    return 256;
+    Q4Plan pl;
+    if (check_attn_q4_args(a) != B2_OK || plan_attn_q4(a, &pl) != B2_OK) return 0;
+    return pl.ws_total;
 }
 
 int b2_paged_attention_q4(const B2PagedAttnQ4Args* a, void* workspace, size_t workspace_bytes, b2_stream_t stream) {
     using namespace b2;
-    const int rc = check_attn_q4_args(a);
+    int rc = check_attn_q4_args(a);
     if (rc != B2_OK || a->batch == 0) return rc;
-    const size_t need = b2_paged_attention_q4_workspace_bytes(a);
-    if (need == 0) return B2_ERR_DEVICE;
-    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need)
+    Q4Plan pl;
+    rc = plan_attn_q4(a, &pl);
+    if (rc != B2_OK) return rc;
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < pl.ws_total)
         return fail(B2_ERR_WORKSPACE, "workspace NULL, not 16-byte aligned or smaller than b2_paged_attention_q4_workspace_bytes");
     Q4AttnParams p;
     p.q = a->q;
@@ -1748,11 +1787,17 @@ int b2_paged_attention_q4(const B2PagedAttnQ4Args* a, void* workspace, size_t wo
     p.window = a->window;
     p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
     p.softcap = a->softcap;
+    p.stages = pl.stages;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    p.ws_count = reinterpret_cast<unsigned*>(ws);
+    p.ws_ml = reinterpret_cast<float2*>(ws + pl.ws_count);
+    p.ws_acc = reinterpret_cast<float*>(ws + pl.ws_count + pl.ws_ml);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->out_dtype == B2_F32)
-        return a->dtype == B2_F16 ? launch_attn_q4<__half, float>(a, p, s) : launch_attn_q4<__nv_bfloat16, float>(a, p, s);
-    return a->dtype == B2_F16 ? launch_attn_q4<__half, __half>(a, p, s)
-                              : launch_attn_q4<__nv_bfloat16, __nv_bfloat16>(a, p, s);
+        return a->dtype == B2_F16 ? launch_attn_q4<__half, float>(a, pl, p, s)
+                                  : launch_attn_q4<__nv_bfloat16, float>(a, pl, p, s);
+    return a->dtype == B2_F16 ? launch_attn_q4<__half, __half>(a, pl, p, s)
+                              : launch_attn_q4<__nv_bfloat16, __nv_bfloat16>(a, pl, p, s);
 }
 
 }  // extern "C"
