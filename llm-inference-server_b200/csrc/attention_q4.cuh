@@ -58,11 +58,11 @@ struct Q4AttnParams {
     float2* ws_ml;       // [2 grid][group]
     float* ws_acc;       // [2 grid][group][head_dim]
     int batch, n_head, n_kv_head, group, mbps, layer_idx, n_layer, num_blocks, window;
-    int stages;
+    int stages, stages_log2;
     float scale, softcap;
 };
 
-constexpr int kQ4Warps = 8;
+constexpr int kQ4Warps = 6;
 constexpr int kQ4Threads = 32 * kQ4Warps;
 constexpr int kQ4CtasPerSm = 2;
 constexpr int kQ4MaxGroup = 8;
@@ -92,15 +92,14 @@ __device__ __forceinline__ int q4_blocks(int first, int n) {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 
@@ -112,16 +111,20 @@ __device__ __forceinline__ float2 half2_floats(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// G words from shared memory (G = 2 or 4).
-template <int G>
-__device__ __forceinline__ void ld_words(const uint8_t* p, uint32_t (&w)[G]) {
-    if constexpr (G == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        w[0] = v.x, w[1] = v.y;
-    }
+// N words from shared memory (volatile: they stay between the waits for a stage and its refill).
+template <int N>
+__device__ __forceinline__ void ld_words(uint32_t at, uint32_t (&w)[N]) {
+    if constexpr (N == 4)
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+    else if constexpr (N == 2)
+        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+    else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(at));
+}
+__device__ __forceinline__ uint32_t ld_word(uint32_t at) {
+    uint32_t w[1];
+    ld_words<1>(at, w);
+    return w[0];
 }
 
 // One item's running state in a warp.  Lane = 4 r + i.
@@ -204,39 +207,62 @@ __device__ __forceinline__ void q4_start(const Q4AttnParams& p, int b, int hk, Q
     }
 }
 
-// One chunk of 16 tokens, positions blk * 16 on, keys [first, n) visible.
+// What a lane reads of a chunk, as byte offsets.
 template <int DH>
-__device__ __forceinline__ void q4_chunk(const Q4AttnParams& p, uint8_t* stage, int blk, int first, int n,
-                                         Q4State<DH>& st) {
+struct Q4Lane {
+    using C = Q4Chunk<DH>;
+    // Token of product row r (and r + 8: 8 later), and of product columns 2i and 2i + 1 (and 8
+    // later).  Chosen so that the rows' K words, the lanes' V words and all params are read
+    // without bank conflicts.
+    int tk;
+    uint32_t k, kp, va, vb, ma, mb;
+    __device__ __forceinline__ Q4Lane() {
+        const int lane = threadIdx.x & 31, r = lane >> 2, i = lane & 3;
+        tk = (r & 1) ? 4 + ((r >> 1) ^ 3) : r >> 1;
+        const int ta = i, tb = 4 + (i ^ 3);
+        k = C::k_word(tk, i, 0);
+        kp = C::kKParams + C::param(tk, 0);
+        va = C::v_unit(ta, r, 0);
+        vb = C::v_unit(tb, r, 0);
+        ma = C::kVParams + C::param(ta, r & (C::kGroups - 1));
+        mb = C::kVParams + C::param(tb, r & (C::kGroups - 1));
+    }
+};
+
+// Two chunks of 16 tokens at shared addresses stage[0] and stage[1], positions blk * 16 on and 16
+// later, keys [first, n) visible.  Two at a time: their products are independent, and the
+// softmax's bookkeeping is paid once.  Where the warp has only one chunk left, stage[1] is stage[0]
+// and n ends at the first chunk: a masked token's weight is 0, its codes and steps are finite.
+template <int DH>
+__device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>& at, const uint32_t (&stage)[2], int blk,
+                                        int first, int n, int last, Q4State<DH>& st) {
     using C = Q4Chunk<DH>;
     constexpr int G = DH / 32;
     constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
-    const int lane = threadIdx.x & 31, r = lane >> 2, i = lane & 3;
-    // Token of product row r (and r + 8: 8 later).  Chosen so that the rows' K words,
-    // the lanes' V words and all params are read without bank conflicts.
-    const int tk = (r & 1) ? 4 + ((r >> 1) ^ 3) : r >> 1;
-    const int ta = i, tb = 4 + (i ^ 3);  // V: product columns 2i and 2i + 1
-    const bool edge = blk * kBlockTokens < first || blk * kBlockTokens + kBlockTokens > n;
+    const int pos = blk * kBlockTokens;
+    const bool edge = pos < first || pos + 2 * kBlockTokens > n;
     if (edge) {
         // What masked tokens hold may be anything, NaN included: 0 * NaN must not reach the sums.
-        if (lane < kBlockTokens) {
-            const int j = blk * kBlockTokens + lane;
-            if (j < first || j >= n) {
+        const int lane = threadIdx.x & 31;
+        const int j = pos + lane;
+        if ((j < first || j >= n) && (lane < kBlockTokens || stage[1] != stage[0])) {
+            const uint32_t to = stage[lane >> 4] + C::kVParams + C::param(lane & 15, 0);
 #pragma unroll
-                for (int g = 0; g < G; ++g) *reinterpret_cast<uint32_t*>(stage + C::kVParams + C::param(lane, g)) = 0;
-            }
+            for (int g = 0; g < G; ++g) asm volatile("st.shared.u32 [%0], %1;" ::"r"(to + 4 * g), "r"(0) : "memory");
         }
         // these generic writes come before the copy that refills the stage
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
     }
-    float x[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};  // [token tk, tk + 8][head 2i, 2i + 1]
-    {
+    float x[4][2];  // [tokens tk, tk + 8 of chunk 0, of chunk 1][head 2i, 2i + 1]
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
         uint32_t ka[G], kb[G], pa[G], pb[G];
-        ld_words<G>(stage + C::k_word(tk, i, 0), ka);
-        ld_words<G>(stage + C::k_word(tk + 8, i, 0), kb);
-        ld_words<G>(stage + C::kKParams + C::param(tk, 0), pa);
-        ld_words<G>(stage + C::kKParams + C::param(tk + 8, 0), pb);
+        ld_words<G>(stage[u] + at.k, ka);
+        ld_words<G>(stage[u] + at.k + 8 * (DH / 2), kb);
+        ld_words<G>(stage[u] + at.kp, pa);
+        ld_words<G>(stage[u] + at.kp + 8 * 4 * G, pb);
+        x[2 * u][0] = x[2 * u][1] = x[2 * u + 1][0] = x[2 * u + 1][1] = 0.0f;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -247,55 +273,55 @@ __device__ __forceinline__ void q4_chunk(const Q4AttnParams& p, uint8_t* stage, 
             const float ma = fmaf(-8.0f, a.y, a.x), mb = fmaf(-8.0f, b.y, b.x);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                x[0][h] = fmaf(a.y, c[h], fmaf(ma, st.qs[g][h], x[0][h]));
-                x[1][h] = fmaf(b.y, c[2 + h], fmaf(mb, st.qs[g][h], x[1][h]));
+                x[2 * u][h] = fmaf(a.y, c[h], fmaf(ma, st.qs[g][h], x[2 * u][h]));
+                x[2 * u + 1][h] = fmaf(b.y, c[2 + h], fmaf(mb, st.qs[g][h], x[2 * u + 1][h]));
             }
         }
     }
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int h = 0; h < 2; ++h) x[t][h] *= st.sc[h];
     if (p.softcap > 0.0f) {
         const float cap = p.softcap * kLog2e;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h)  // tanh(y) = 1 - 2 / (1 + e^2y): 2^-23 absolute, to be multiplied by the cap
                 x[t][h] = cap - __fdividef(2.0f * cap, 1.0f + ex2_approx(x[t][h]));
     }
     if (p.slopes != nullptr) {
-        const float d = static_cast<float>(blk * kBlockTokens + tk - (n - 1));
+        const float d = static_cast<float>(pos + at.tk - last);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            x[0][h] = fmaf(st.slope[h], d, x[0][h]);
-            x[1][h] = fmaf(st.slope[h], d + 8.0f, x[1][h]);
-        }
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[t][h] = fmaf(st.slope[h], d + 8.0f * t, x[t][h]);
     }
     if (edge) {
-        const int j = blk * kBlockTokens + tk;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (j < first || j >= n) x[0][h] = -INFINITY;
-            if (j + 8 < first || j + 8 >= n) x[1][h] = -INFINITY;
+        for (int t = 0; t < 4; ++t) {
+            const int j = pos + at.tk + 8 * t;
+            if (j < first || j >= n) x[t][0] = x[t][1] = -INFINITY;
         }
     }
-    uint32_t va[G], vb[G];  // V params of tokens tk, tk + 8
-    ld_words<G>(stage + C::kVParams + C::param(tk, 0), va);
-    ld_words<G>(stage + C::kVParams + C::param(tk + 8, 0), vb);
+    uint32_t vp[4][G];  // V params of the four tokens
+#pragma unroll
+    for (int t = 0; t < 4; ++t) ld_words<G>(stage[t >> 1] + at.kp + C::kV + (t & 1) * 8 * 4 * G, vp[t]);
     float top[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) top[h] = fmaxf(x[0][h], x[1][h]);
+    for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(x[0][h], x[1][h]), fmaxf(x[2][h], x[3][h]));
     uint32_t s_top = 0;
 #pragma unroll
-    for (int g = 0; g < G; ++g) s_top = max(s_top, max(va[g], vb[g]));
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int g = 0; g < G; g += 2) s_top = __vimax3_u32(s_top, vp[t][g], vp[t][g + 1]);
     if (__any_sync(0xffffffffu, top[0] - 4.0f > st.ref[0] || top[1] - 4.0f > st.ref[1] || s_top >= st.s_limit)) {
         s_top = 0;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {  // NaN and infinite steps do not count
-            if (va[g] < 0x7c000000u) s_top = max(s_top, va[g]);
-            if (vb[g] < 0x7c000000u) s_top = max(s_top, vb[g]);
-        }
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int g = 0; g < G; ++g)  // NaN and infinite steps do not count
+                if (vp[t][g] < 0x7c000000u) s_top = max(s_top, vp[t][g]);
         s_top = __reduce_max_sync(0xffffffffu, s_top);
         const int k = min(st.k, 18 - static_cast<int>(s_top >> 26));  // s 2^k < 2^4
         const float by = __uint_as_float(static_cast<uint32_t>(127 + k - st.k) << 23);
@@ -319,52 +345,47 @@ __device__ __forceinline__ void q4_chunk(const Q4AttnParams& p, uint8_t* stage, 
                 }
         }
     }
-    float w[2][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        w[0][h] = ex2_approx(x[0][h] - st.ref[h]);
-        w[1][h] = ex2_approx(x[1][h] - st.ref[h]);
-        st.l[h] += w[0][h] + w[1][h];
-    }
-    {  // sum p m: A rows = groups (rows from G on repeat them, unused)
-        const uint8_t* pm = stage + C::kVParams + (r & (G - 1)) * 4;
-        const uint32_t m0 = *reinterpret_cast<const uint32_t*>(pm + C::param(ta, 0));
-        const uint32_t m1 = *reinterpret_cast<const uint32_t*>(pm + C::param(tb, 0));
-        const uint32_t m2 = *reinterpret_cast<const uint32_t*>(pm + C::param(ta + 8, 0));
-        const uint32_t m3 = *reinterpret_cast<const uint32_t*>(pm + C::param(tb + 8, 0));
-        const uint32_t b0 = transpose8x8(half2_bits(w[0][0], w[0][1]));
-        const uint32_t b1 = transpose8x8(half2_bits(w[1][0], w[1][1]));
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            x[t][h] = ex2_approx(x[t][h] - st.ref[h]);  // the weights from here on
+            st.l[h] += x[t][h];
+        }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {  // sum p m: A rows = groups (rows from G on repeat them, unused)
+        const uint32_t m0 = ld_word(stage[u] + at.ma), m1 = ld_word(stage[u] + at.mb);
+        const uint32_t m2 = ld_word(stage[u] + at.ma + 8 * 4 * G), m3 = ld_word(stage[u] + at.mb + 8 * 4 * G);
+        const uint32_t b0 = transpose8x8(half2_bits(x[2 * u][0], x[2 * u][1]));
+        const uint32_t b1 = transpose8x8(half2_bits(x[2 * u + 1][0], x[2 * u + 1][1]));
         mma_f16(st.tz, __byte_perm(m0, m1, 0x5410), 0, __byte_perm(m2, m3, 0x5410), 0, b0, b1);
     }
     const float up = __uint_as_float(static_cast<uint32_t>(127 + st.k) << 23);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) w[t][h] *= up;
-    uint32_t v[4][G / 2];  // words of tokens ta, tb, ta + 8, tb + 8: groups 2w (low) and 2w + 1 (high)
+        for (int h = 0; h < 2; ++h) x[t][h] *= up;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const uint8_t* at = stage + C::v_unit((t & 1 ? tb : ta) + (t & 2 ? 8 : 0), r, 0);
-        if constexpr (G == 4) {
-            const uint2 u = *reinterpret_cast<const uint2*>(at);
-            v[t][0] = u.x, v[t][1] = u.y;
-        } else {
-            v[t][0] = *reinterpret_cast<const uint32_t*>(at);
+    for (int u = 0; u < 2; ++u) {
+        uint32_t v[4][G / 2];  // words of product columns 2i, 2i + 1 and 8 later: groups 2w (low) and 2w + 1 (high)
+        ld_words<G / 2>(stage[u] + at.va, v[0]);
+        ld_words<G / 2>(stage[u] + at.vb, v[1]);
+        ld_words<G / 2>(stage[u] + at.va + 256, v[2]);
+        ld_words<G / 2>(stage[u] + at.vb + 256, v[3]);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float sa = half2_floats(vp[2 * u][g]).y, sb = half2_floats(vp[2 * u + 1][g]).y;
+            const uint32_t b0 = transpose8x8(half2_bits(x[2 * u][0] * sa, x[2 * u][1] * sa));
+            const uint32_t b1 = transpose8x8(half2_bits(x[2 * u + 1][0] * sb, x[2 * u + 1][1] * sb));
+            const uint32_t pick = g & 1 ? 0x7632 : 0x5410;
+            const uint32_t u0 = __byte_perm(v[0][g / 2], v[1][g / 2], pick), u1 = __byte_perm(v[2][g / 2], v[3][g / 2], pick);
+            mma_f16(st.acc[g][0], u0 & kLow, u0 & kHigh, u1 & kLow, u1 & kHigh, b0, b1);
+            const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
+            mma_f16(st.acc[g][1], w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh, b0, b1);
+            // -8 in the units of even and odd dims: -8 2^-24 and -8 16 2^-24
+            mma_f16(st.acc[g][0], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
+            mma_f16(st.acc[g][1], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
         }
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-        const float sa = half2_floats(va[g]).y, sb = half2_floats(vb[g]).y;
-        const uint32_t b0 = transpose8x8(half2_bits(w[0][0] * sa, w[0][1] * sa));
-        const uint32_t b1 = transpose8x8(half2_bits(w[1][0] * sb, w[1][1] * sb));
-        const uint32_t pick = g & 1 ? 0x7632 : 0x5410;
-        const uint32_t u0 = __byte_perm(v[0][g / 2], v[1][g / 2], pick), u1 = __byte_perm(v[2][g / 2], v[3][g / 2], pick);
-        mma_f16(st.acc[g][0], u0 & kLow, u0 & kHigh, u1 & kLow, u1 & kHigh, b0, b1);
-        const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
-        mma_f16(st.acc[g][1], w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh, b0, b1);
-        // -8 in the units of even and odd dims: -8 2^-24 and -8 16 2^-24
-        mma_f16(st.acc[g][0], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
-        mma_f16(st.acc[g][1], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
     }
 }
 
@@ -459,9 +480,6 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
     // Lane's chunk of the 32 from `from` on: where it lies and what it is.
     auto locate = [&](unsigned from, unsigned* chunk, int* item, int* blk) {
         const unsigned c = from + lane;
-        *chunk = 0;
-        *item = -1;
-        *blk = 0;
         if (c >= c1) return;
         const int seg = last_at_most(s_seg, kQ4Threads, c);
         unsigned base = s_seg[seg];
@@ -483,26 +501,12 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
         }
         *chunk = static_cast<unsigned>((static_cast<long long>(id) * p.n_layer + p.layer_idx) * p.n_kv_head + h);
     };
+    // Two windows of 32 chunks, a chunk to a lane: the one from window_at on and the one before it.
     unsigned new_chunk = 0, old_chunk = 0;
     int new_item = -1, new_blk = 0, old_item = -1, old_blk = 0;
-    unsigned issued = c0, window_at = c0;  // next chunk to copy; first chunk of the new window of 32
-    auto issue = [&](int stage) {  // all lanes; copies chunk `issued`
-        if (issued == window_at + 32) {
-            old_chunk = new_chunk, old_item = new_item, old_blk = new_blk;
-            window_at = issued;
-            locate(issued, &new_chunk, &new_item, &new_blk);
-        }
-        const unsigned chunk = __shfl_sync(0xffffffffu, new_chunk, issued - window_at);
-        if (lane == 0) {
-            mbar_arrive_expect_tx(bars + stage, C::kBytes);
-            bulk_g2s(ring + stage * C::kBytes, p.pool + static_cast<size_t>(chunk) * C::kBytes, C::kBytes, bars + stage);
-        }
-        ++issued;
-    };
-    if (c0 < c1) {
-        locate(c0, &new_chunk, &new_item, &new_blk);
-        for (int s = 0; s < p.stages && issued < c1; ++s) issue(s);
-    }
+    unsigned window_at = c0 - 32, issued = c0;
+    const unsigned slot_mask = p.stages - 1;
+    const uint32_t ring_at = smem_addr(ring);
 
     Q4State<DH> st;
     int item = -1, first = 0, n = 0, from_blk = 0;
@@ -541,90 +545,128 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
             s_entry[2 * warp + slot] = Q4Entry{item, from - static_cast<unsigned>(from_blk - first / kBlockTokens),
                                                static_cast<unsigned>(nb)};
     };
-    int stage = 0;
-    uint32_t parity = 0;
+    const Q4Lane<DH> offs;
     bool alive = true;
-    unsigned c = c0;
-    for (; c < c1; ++c) {
-        const bool in_new = c >= window_at;
-        const int src = static_cast<int>(in_new ? c - window_at : c - (window_at - 32));
-        const int it = __shfl_sync(0xffffffffu, in_new ? new_item : old_item, src);
-        const int blk = __shfl_sync(0xffffffffu, in_new ? new_blk : old_blk, src);
-        if (it != item) {
+    unsigned c = c0, item_end = c0;
+    int blk = 0;
+    while (c0 < c1) {
+        // Refill the ring: a lane copies its own chunk where that is among the next ones to copy.
+        const unsigned limit = min(c1, c + p.stages);
+        if (limit > window_at + 32) {
+            old_chunk = new_chunk, old_item = new_item, old_blk = new_blk;
+            window_at += 32;
+            locate(window_at, &new_chunk, &new_item, &new_blk);
+        }
+        {
+            const bool in_new = window_at + lane < limit;
+            const unsigned idx = in_new ? window_at + lane : window_at + lane - 32;
+            if (static_cast<int>(idx - issued) >= 0 && idx < limit) {
+                const unsigned slot = (idx - c0) & slot_mask;
+                mbar_arrive_expect_tx(bars + slot, C::kBytes);
+                bulk_g2s(ring + slot * C::kBytes,
+                         p.pool + static_cast<size_t>(in_new ? new_chunk : old_chunk) * C::kBytes, C::kBytes, bars + slot);
+            }
+            issued = limit;
+            __syncwarp();
+        }
+        if (c == item_end) {
             if (item >= 0) end_item(c);
-            item = it;
+            if (c == c1) break;
+            const bool in_new = static_cast<int>(c - window_at) >= 0;
+            const int src = static_cast<int>((c - c0) & 31);
+            item = __shfl_sync(0xffffffffu, in_new ? new_item : old_item, src);
+            blk = __shfl_sync(0xffffffffu, in_new ? new_blk : old_blk, src);
             from = c;
             from_blk = blk;
-            const int b = it / p.n_kv_head;
+            const int b = item / p.n_kv_head;
             unsigned none = 0;
             q4_range(p, b, &first, &n, &none);
-            q4_start<T, DH>(p, b, it - b * p.n_kv_head, st);
+            item_end = min(c1, c + static_cast<unsigned>((n - 1) / kBlockTokens - blk + 1));
+            q4_start<T, DH>(p, b, item - b * p.n_kv_head, st);
         }
-        alive = __all_sync(0xffffffffu, mbar_wait_bounded(bars + stage, parity));
+        const bool two = c + 1 < item_end;
+        const unsigned k0 = c - c0, k1 = two ? k0 + 1 : k0;
+        const unsigned s0 = k0 & slot_mask, s1 = k1 & slot_mask;
+        alive = __all_sync(0xffffffffu, mbar_wait_bounded(bars + s0, (k0 >> p.stages_log2) & 1) &&
+                                            mbar_wait_bounded(bars + s1, (k1 >> p.stages_log2) & 1));
         if (!alive) break;
-        q4_chunk<DH>(p, ring + stage * C::kBytes, blk, first, n, st);
-        __syncwarp();  // every lane is done with the stage
-        if (issued < c1) issue(stage);
-        if (++stage == p.stages) {
-            stage = 0;
-            parity ^= 1;
-        }
+        const uint32_t at[2] = {ring_at + s0 * C::kBytes, ring_at + s1 * C::kBytes};
+        q4_step<DH>(p, offs, at, blk, first, two ? n : min(n, (blk + 1) * kBlockTokens), n - 1, st);
+        __syncwarp();  // every lane is done with the slots
+        c += two ? 2 : 1;
+        blk += two ? 2 : 1;
     }
-    if (alive) {
-        if (item >= 0) end_item(c1);
-    } else {  // the copies in flight end before this CTA's shared memory goes
+    if (!alive) {  // the copies in flight end before this CTA's shared memory goes
         err |= B2_DEVERR_TIMEOUT;
-        for (; c < issued; ++c) {
-            mbar_wait_bounded(bars + stage, parity);
-            if (++stage == p.stages) {
-                stage = 0;
-                parity ^= 1;
-            }
-        }
+        for (; c < issued; ++c) mbar_wait_bounded(bars + ((c - c0) & slot_mask), ((c - c0) >> p.stages_log2) & 1);
+    }
+    // Sequences without a visible key.
+    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        int lo, len;
+        unsigned none = 0;
+        q4_range(p, b, &lo, &len, &none);
+        if (lo < len) continue;
+        OutT* row = static_cast<OutT*>(p.out) + static_cast<size_t>(b) * p.n_head * DH;
+        for (int e = tid * 4; e < p.n_head * DH; e += kQ4Threads * 4) q4_store4<OutT>(row + e, 0.0f, 0.0f, 0.0f, 0.0f);
     }
     __syncthreads();
 
-    // Pieces of one item lie in consecutive entries; the warp that holds the first of them merges them.
+    // Pieces of one item lie in consecutive entries (a run).  Every warp sees all entries in its
+    // lanes and takes every kQ4Warps-th (run, head).
     const unsigned cta0 = active ? bound(blockIdx.x * kQ4Warps) : 0, cta1 = active ? bound((blockIdx.x + 1) * kQ4Warps) : 0;
-    for (int slot = 0; slot < 2; ++slot) {
-        const int e0 = 2 * warp + slot;
-        const Q4Entry en = s_entry[e0];
-        if (en.item < 0) continue;
-        int prev = e0 - 1;
-        while (prev >= 0 && s_entry[prev].item < 0) --prev;
-        if (prev >= 0 && s_entry[prev].item == en.item) continue;
-        const bool whole = en.start >= cta0 && en.start + en.count <= cta1;
-        const int open = en.start >= cta0 ? 1 : 0;
-        const size_t at = static_cast<size_t>(blockIdx.x) * 2 + open;
-        const int b = en.item / p.n_kv_head, hk = en.item - b * p.n_kv_head;
-        for (int h = 0; h < p.group; ++h) {
-            float top = -FLT_MAX;
-            for (int e = e0; e < 2 * kQ4Warps; ++e)
-                if (s_entry[e].item == en.item) top = fmaxf(top, piece_at(e >> 1, e & 1)[p.group * DH + 2 * h]);
-            float l = 0.0f;
+    {
+        const int it = lane < 2 * kQ4Warps ? s_entry[lane].item : -1;
+        const unsigned valid = __ballot_sync(0xffffffffu, it >= 0);
+        const unsigned before = valid & ((1u << lane) - 1);
+        const int prev = __shfl_sync(0xffffffffu, it, before != 0 ? 31 - __clz(before) : lane);
+        const unsigned starts = __ballot_sync(0xffffffffu, it >= 0 && (before == 0 || prev != it));
+        const int tasks = __popc(starts) * p.group;
+#pragma unroll 1
+        for (int task = warp; task < tasks; task += kQ4Warps) {
+            const int run = task / p.group, h = task - run * p.group;
+            unsigned from_run = starts;
+            for (int skip = run; skip > 0; --skip) from_run &= from_run - 1;
+            const int e0 = __ffs(from_run) - 1;
+            const unsigned later = starts & ~((2u << e0) - 1);
+            const unsigned run_bits = valid & ~((1u << e0) - 1) & (later != 0 ? (later & (0u - later)) - 1 : 0xffffffffu);
+            const Q4Entry en = s_entry[e0];
+            const float* ml = piece_at(min(lane, 2 * kQ4Warps - 1) >> 1, lane & 1) + p.group * DH + 2 * h;
+            const bool in_run = run_bits >> lane & 1u;
+            const float ref = in_run ? ml[0] : -FLT_MAX;
+            float top = ref;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float f = in_run ? ex2_approx(ref - top) : 0.0f;
+            float l = in_run ? f * ml[1] : 0.0f;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
             float sum[G];
 #pragma unroll
             for (int g = 0; g < G; ++g) sum[g] = 0.0f;
-            for (int e = e0; e < 2 * kQ4Warps; ++e)
-                if (s_entry[e].item == en.item) {
-                    const float* pc = piece_at(e >> 1, e & 1);
-                    const float f = ex2_approx(pc[p.group * DH + 2 * h] - top);
-                    l = fmaf(pc[p.group * DH + 2 * h + 1], f, l);
+            for (unsigned left = run_bits; left != 0; left &= left - 1) {
+                const int e = __ffs(left) - 1;
+                const float* pc = piece_at(e >> 1, e & 1) + h * DH + lane;
+                const float fe = __shfl_sync(0xffffffffu, f, e);
 #pragma unroll
-                    for (int g = 0; g < G; ++g) sum[g] = fmaf(pc[h * DH + 32 * g + lane], f, sum[g]);
-                }
-            if (whole) {
+                for (int g = 0; g < G; ++g) sum[g] = fmaf(pc[32 * g], fe, sum[g]);
+            }
+            if (en.start >= cta0 && en.start + en.count <= cta1) {
+                const int b = en.item / p.n_kv_head, hk = en.item - b * p.n_kv_head;
                 const float inv = 1.0f / l;
                 OutT* row = static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH;
 #pragma unroll
                 for (int g = 0; g < G; ++g) row[32 * g + lane] = Elem<OutT>::from_f(sum[g] * inv);
             } else {
+                const int open = en.start >= cta0 ? 1 : 0;
+                const size_t at = (static_cast<size_t>(blockIdx.x) * 2 + open) * p.group + h;
 #pragma unroll
-                for (int g = 0; g < G; ++g) __stcg(p.ws_acc + (at * p.group + h) * DH + 32 * g + lane, sum[g]);
-                if (lane == 0) __stcg(p.ws_ml + at * p.group + h, make_float2(top, l));
+                for (int g = 0; g < G; ++g) __stcg(p.ws_acc + at * DH + 32 * g + lane, sum[g]);
+                if (lane == 0) {
+                    __stcg(p.ws_ml + at, make_float2(top, l));
+                    if (h == 0) s_open[open] = en;
+                }
             }
         }
-        if (!whole && lane == 0) s_open[open] = en;
     }
     __syncthreads();
 
@@ -646,42 +688,75 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
         }
     }
     __syncthreads();
+#pragma unroll 1
     for (int open = 0; open < 2; ++open) {
         if (!s_last[open]) continue;
         const Q4Entry en = s_open[open];
-        const unsigned f = cta_of(en.start), last = cta_of(en.start + en.count - 1);
+        const int f = static_cast<int>(cta_of(en.start));
+        const int parts_n = static_cast<int>(cta_of(en.start + en.count - 1)) - f + 1;
         const int b = en.item / p.n_kv_head, hk = en.item - b * p.n_kv_head;
-        for (int e = tid * 4; e < p.group * DH; e += kQ4Threads * 4) {
-            const int h = e / DH, d = e % DH;
-            float top = -FLT_MAX, l = 0.0f;
-            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (unsigned j = f; j <= last; ++j)
-                top = fmaxf(top, __ldcg(p.ws_ml + (2ull * j + (j == f ? 1 : 0)) * p.group + h).x);
-#pragma unroll 4
-            for (unsigned j = f; j <= last; ++j) {
-                const size_t at = (2ull * j + (j == f ? 1 : 0)) * p.group + h;
-                const float2 ml = __ldcg(p.ws_ml + at);
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + at * DH + d));
+        // workspace row of part j and head h: the item's first CTA wrote its slot 1, the others slot 0
+        auto row_of = [&](int j, int h) { return (2ull * (f + j) + (j == 0 ? 1 : 0)) * p.group + h; };
+        // the parts' weights and l, per head, in the (drained) rings: [group][parts] and [group]
+        float* weight = reinterpret_cast<float*>(smem);
+        float* denom = weight + p.group * parts_n;
+        float4* partial = reinterpret_cast<float4*>(weight + (p.group * (parts_n + 1) + 3) / 4 * 4);
+        for (int h = warp; h < p.group; h += kQ4Warps) {
+            float top = -FLT_MAX;
+            for (int j = lane; j < parts_n; j += 32) top = fmaxf(top, __ldcg(p.ws_ml + row_of(j, h)).x);
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            float l = 0.0f;
+            for (int j = lane; j < parts_n; j += 32) {
+                const float2 ml = __ldcg(p.ws_ml + row_of(j, h));
                 const float w = ex2_approx(ml.x - top);
+                weight[h * parts_n + j] = w;
                 l = fmaf(ml.y, w, l);
+            }
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+            if (lane == 0) denom[h] = l;
+        }
+        __syncthreads();
+        // (head, 4 dims) to a thread; spare threads take shares of the parts
+        const int quads = p.group * DH / 4;
+        const int shares = max(1, kQ4Threads / quads);
+        for (int e = tid; e < quads * shares; e += kQ4Threads) {
+            const int share = e / quads, q = e - share * quads;
+            const int h = q / (DH / 4), d = q % (DH / 4) * 4;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for (int j = share; j < parts_n; j += shares) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + row_of(j, h) * DH + d));
+                const float w = weight[h * parts_n + j];
                 sum.x = fmaf(v.x, w, sum.x);
                 sum.y = fmaf(v.y, w, sum.y);
                 sum.z = fmaf(v.z, w, sum.z);
                 sum.w = fmaf(v.w, w, sum.w);
             }
-            const float inv = 1.0f / l;
-            q4_store4<OutT>(static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH + d,
-                            sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            if (shares > 1) {
+                partial[e] = sum;
+            } else {
+                const float inv = 1.0f / denom[h];
+                q4_store4<OutT>(static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH + d,
+                                sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            }
         }
-    }
-    // Sequences without a visible key.
-    for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-        int lo, len;
-        unsigned none = 0;
-        q4_range(p, b, &lo, &len, &none);
-        if (lo < len) continue;
-        OutT* row = static_cast<OutT*>(p.out) + static_cast<size_t>(b) * p.n_head * DH;
-        for (int e = tid * 4; e < p.n_head * DH; e += kQ4Threads * 4) q4_store4<OutT>(row + e, 0.0f, 0.0f, 0.0f, 0.0f);
+        if (shares > 1) {
+            __syncthreads();
+            if (tid < quads) {
+                const int h = tid / (DH / 4), d = tid % (DH / 4) * 4;
+                float4 sum = partial[tid];
+                for (int s = 1; s < shares; ++s) {
+                    const float4 v = partial[s * quads + tid];
+                    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+                }
+                const float inv = 1.0f / denom[h];
+                q4_store4<OutT>(static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH + d,
+                                sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            }
+        }
+        __syncthreads();  // the shared arrays serve the next item
     }
     if (err != 0) flag_error(err);
 }

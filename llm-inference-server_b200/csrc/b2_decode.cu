@@ -1656,7 +1656,7 @@ struct Q4Plan {
     size_t ws_count = 0, ws_ml = 0, ws_total = 0;  // [counters][(R, l)][sums]
 };
 
-// Two CTAs per SM; as many ring stages (up to 8) as their half of the shared memory holds.
+// Two CTAs per SM; as many ring stages (2, 4 or 8) as their half of the shared memory holds.
 int plan_attn_q4(const B2PagedAttnQ4Args* a, Q4Plan* pl) {
     int dev = -1;
     const DeviceInfo di = device_info(&dev);
@@ -1665,7 +1665,8 @@ int plan_attn_q4(const B2PagedAttnQ4Args* a, Q4Plan* pl) {
     const int pieces = kQ4Warps * q4_piece_bytes(group, a->head_dim);
     const int per_stage = kQ4Warps * (20 * a->head_dim + 8);
     const int room = di.smem_per_sm / kQ4CtasPerSm - 1024 - 2048;  // reserved and static shared memory
-    pl->stages = std::min(8, (room - pieces) / per_stage);
+    const int fit = (room - pieces) / per_stage;
+    pl->stages = fit >= 8 ? 8 : fit >= 4 ? 4 : fit >= 2 ? 2 : 0;
     // a warp's last piece is kept in its drained ring
     if (pl->stages < 2 || pl->stages * 20 * a->head_dim < q4_piece_bytes(group, a->head_dim))
         return fail(B2_ERR_UNSUPPORTED, "4-bit attention: shared memory");
@@ -1788,6 +1789,7 @@ int b2_paged_attention_q4(const B2PagedAttnQ4Args* a, void* workspace, size_t wo
     p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
     p.softcap = a->softcap;
     p.stages = pl.stages;
+    p.stages_log2 = pl.stages == 8 ? 3 : pl.stages == 4 ? 2 : 1;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.ws_count = reinterpret_cast<unsigned*>(ws);
     p.ws_ml = reinterpret_cast<float2*>(ws + pl.ws_count);
