@@ -59,6 +59,7 @@ struct Q4AttnParams {
     float* ws_acc;       // [2 grid][group][head_dim]
     int batch, n_head, n_kv_head, group, mbps, layer_idx, n_layer, num_blocks, window;
     int stages, stages_log2;
+    unsigned kv_mul, kv_shift;  // n / n_kv_head = n * kv_mul >> kv_shift for n < 2^31
     float scale, softcap;
 };
 
@@ -83,6 +84,10 @@ __device__ __forceinline__ void q4_range(const Q4AttnParams& p, int b, int* firs
     if (p.window > 0) lo = max(lo, len - p.window);
     *first = min(lo, len);
     *n = len;
+}
+
+__device__ __forceinline__ int q4_sequence(const Q4AttnParams& p, int item) {
+    return static_cast<int>(static_cast<unsigned long long>(static_cast<unsigned>(item)) * p.kv_mul >> p.kv_shift);
 }
 
 // Blocks that hold visible keys.
@@ -437,6 +442,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
     __shared__ Q4Entry s_entry[2 * kQ4Warps];
     __shared__ Q4Entry s_open[2];  // items of this CTA that other CTAs hold parts of
     __shared__ int s_last[2];
+    __shared__ int2 s_parts[2];  // their first CTA and number of CTAs
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane & 3, r = lane >> 2;
     const int piece_bytes = q4_piece_bytes(p.group, DH);
     uint8_t* ring = smem + static_cast<size_t>(warp) * p.stages * C::kBytes;
@@ -448,6 +454,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
                                                   : smem + static_cast<size_t>(w) * p.stages * C::kBytes);
     };
     if (lane == 0) {
+#pragma unroll 1
         for (int s = 0; s < p.stages; ++s) mbar_init(bars + s, 1);
         fence_mbar_init();
     }
@@ -460,6 +467,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
     unsigned err = 0;
     const int per = (p.batch + kQ4Threads - 1) / kQ4Threads;
     unsigned mine = 0;
+#pragma unroll 1
     for (int b = min(tid * per, p.batch); b < min((tid + 1) * per, p.batch); ++b) {
         int first, n;
         q4_range(p, b, &first, &n, &err);
@@ -471,8 +479,9 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
     __syncthreads();
     // Fewer CTAs than launched where a warp would get less than a chunk.
     const unsigned ctas = max(1u, min(gridDim.x, (total + kQ4Warps - 1) / kQ4Warps));
-    const unsigned long long parts = static_cast<unsigned long long>(ctas) * kQ4Warps;
-    auto bound = [&](unsigned part) { return static_cast<unsigned>(static_cast<unsigned long long>(total) * part / parts); };
+    // Part (warp) i of the list: `each` chunks, one more for the first `more` parts.
+    const unsigned parts = ctas * kQ4Warps, each = total / parts, more = total - each * parts;
+    auto bound = [&](unsigned part) { return part * each + min(part, more); };
     const bool active = blockIdx.x < ctas;
     const unsigned c0 = active ? bound(blockIdx.x * kQ4Warps + warp) : 0;
     const unsigned c1 = active ? bound(blockIdx.x * kQ4Warps + warp + 1) : 0;
@@ -485,6 +494,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
         unsigned base = s_seg[seg];
         int b = seg * per, first, n, nb;
         unsigned none = 0;
+#pragma unroll 1
         for (;; ++b) {
             q4_range(p, b, &first, &n, &none);
             nb = q4_blocks(first, n);
@@ -515,7 +525,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
     auto end_item = [&](unsigned upto) {
         float o[2][G][4], l[2];
         q4_finish<DH>(st, o, l);
-        const int b = item / p.n_kv_head, hk = item - b * p.n_kv_head;
+        const int b = q4_sequence(p, item), hk = item - b * p.n_kv_head;
         const int nb = q4_blocks(first, n);
         if (upto - from == static_cast<unsigned>(nb)) {
 #pragma unroll
@@ -578,7 +588,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
             blk = __shfl_sync(0xffffffffu, in_new ? new_blk : old_blk, src);
             from = c;
             from_blk = blk;
-            const int b = item / p.n_kv_head;
+            const int b = q4_sequence(p, item);
             unsigned none = 0;
             q4_range(p, b, &first, &n, &none);
             item_end = min(c1, c + static_cast<unsigned>((n - 1) / kBlockTokens - blk + 1));
@@ -598,15 +608,18 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
     }
     if (!alive) {  // the copies in flight end before this CTA's shared memory goes
         err |= B2_DEVERR_TIMEOUT;
+#pragma unroll 1
         for (; c < issued; ++c) mbar_wait_bounded(bars + ((c - c0) & slot_mask), ((c - c0) >> p.stages_log2) & 1);
     }
     // Sequences without a visible key.
+#pragma unroll 1
     for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
         int lo, len;
         unsigned none = 0;
         q4_range(p, b, &lo, &len, &none);
         if (lo < len) continue;
         OutT* row = static_cast<OutT*>(p.out) + static_cast<size_t>(b) * p.n_head * DH;
+#pragma unroll 1
         for (int e = tid * 4; e < p.n_head * DH; e += kQ4Threads * 4) q4_store4<OutT>(row + e, 0.0f, 0.0f, 0.0f, 0.0f);
     }
     __syncthreads();
@@ -625,6 +638,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
         for (int task = warp; task < tasks; task += kQ4Warps) {
             const int run = task / p.group, h = task - run * p.group;
             unsigned from_run = starts;
+#pragma unroll 1
             for (int skip = run; skip > 0; --skip) from_run &= from_run - 1;
             const int e0 = __ffs(from_run) - 1;
             const unsigned later = starts & ~((2u << e0) - 1);
@@ -643,6 +657,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
             float sum[G];
 #pragma unroll
             for (int g = 0; g < G; ++g) sum[g] = 0.0f;
+#pragma unroll 1
             for (unsigned left = run_bits; left != 0; left &= left - 1) {
                 const int e = __ffs(left) - 1;
                 const float* pc = piece_at(e >> 1, e & 1) + h * DH + lane;
@@ -651,7 +666,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
                 for (int g = 0; g < G; ++g) sum[g] = fmaf(pc[32 * g], fe, sum[g]);
             }
             if (en.start >= cta0 && en.start + en.count <= cta1) {
-                const int b = en.item / p.n_kv_head, hk = en.item - b * p.n_kv_head;
+                const int b = q4_sequence(p, en.item), hk = en.item - b * p.n_kv_head;
                 const float inv = 1.0f / l;
                 OutT* row = static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH;
 #pragma unroll
@@ -672,18 +687,20 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
 
     // Items over several CTAs: the last CTA to arrive merges, in CTA order.
     auto cta_of = [&](unsigned chunk) {
-        return static_cast<unsigned>(((chunk + 1ull) * ctas - 1) / total);
+        const unsigned split = more * (each + 1);
+        return (chunk < split ? chunk / (each + 1) : more + (chunk - split) / each) / kQ4Warps;
     };
     if (tid < 2) {
         s_last[tid] = 0;
         if (s_open[tid].item >= 0) {
             const unsigned f = cta_of(s_open[tid].start), last = cta_of(s_open[tid].start + s_open[tid].count - 1);
-            __threadfence();
-            const unsigned before = atomicAdd(p.ws_count + f, 1u);
+            s_parts[tid] = make_int2(static_cast<int>(f), static_cast<int>(last - f + 1));
+            // release: this CTA's parts (ordered before by the barrier); acquire: the others'
+            unsigned before;
+            asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(p.ws_count + f) : "memory");
             if (before == last - f) {
                 s_last[tid] = 1;
                 p.ws_count[f] = 0;
-                __threadfence();
             }
         }
     }
@@ -692,26 +709,33 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
     for (int open = 0; open < 2; ++open) {
         if (!s_last[open]) continue;
         const Q4Entry en = s_open[open];
-        const int f = static_cast<int>(cta_of(en.start));
-        const int parts_n = static_cast<int>(cta_of(en.start + en.count - 1)) - f + 1;
-        const int b = en.item / p.n_kv_head, hk = en.item - b * p.n_kv_head;
+        const int f = s_parts[open].x, parts_n = s_parts[open].y;
+        const int b = q4_sequence(p, en.item), hk = en.item - b * p.n_kv_head;
         // workspace row of part j and head h: the item's first CTA wrote its slot 1, the others slot 0
-        auto row_of = [&](int j, int h) { return (2ull * (f + j) + (j == 0 ? 1 : 0)) * p.group + h; };
+        auto row_of = [&](int j, int h) { return (2 * (f + j) + (j == 0 ? 1 : 0)) * p.group + h; };
         // the parts' weights and l, per head, in the (drained) rings: [group][parts] and [group]
         float* weight = reinterpret_cast<float*>(smem);
         float* denom = weight + p.group * parts_n;
         float4* partial = reinterpret_cast<float4*>(weight + (p.group * (parts_n + 1) + 3) / 4 * 4);
+#pragma unroll 1
         for (int h = warp; h < p.group; h += kQ4Warps) {
-            float top = -FLT_MAX;
-            for (int j = lane; j < parts_n; j += 32) top = fmaxf(top, __ldcg(p.ws_ml + row_of(j, h)).x);
+            // a lane keeps its first two parts; beyond 64 parts they are read twice
+            float2 ml[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                ml[k] = lane + 32 * k < parts_n ? __ldcg(p.ws_ml + row_of(lane + 32 * k, h)) : make_float2(-FLT_MAX, 0.0f);
+            float top = fmaxf(ml[0].x, ml[1].x);
+#pragma unroll 1
+            for (int j = lane + 64; j < parts_n; j += 32) top = fmaxf(top, __ldcg(p.ws_ml + row_of(j, h)).x);
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             float l = 0.0f;
-            for (int j = lane; j < parts_n; j += 32) {
-                const float2 ml = __ldcg(p.ws_ml + row_of(j, h));
-                const float w = ex2_approx(ml.x - top);
+#pragma unroll 1
+            for (int j = lane, k = 0; j < parts_n; j += 32, ++k) {
+                const float2 v = k == 0 ? ml[0] : k == 1 ? ml[1] : __ldcg(p.ws_ml + row_of(j, h));
+                const float w = ex2_approx(v.x - top);
                 weight[h * parts_n + j] = w;
-                l = fmaf(ml.y, w, l);
+                l = fmaf(v.y, w, l);
             }
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
@@ -721,13 +745,14 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
         // (head, 4 dims) to a thread; spare threads take shares of the parts
         const int quads = p.group * DH / 4;
         const int shares = max(1, kQ4Threads / quads);
+#pragma unroll 1
         for (int e = tid; e < quads * shares; e += kQ4Threads) {
             const int share = e / quads, q = e - share * quads;
             const int h = q / (DH / 4), d = q % (DH / 4) * 4;
             float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
+#pragma unroll 8
             for (int j = share; j < parts_n; j += shares) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + row_of(j, h) * DH + d));
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + static_cast<size_t>(row_of(j, h)) * DH + d));
                 const float w = weight[h * parts_n + j];
                 sum.x = fmaf(v.x, w, sum.x);
                 sum.y = fmaf(v.y, w, sum.y);
@@ -747,6 +772,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
             if (tid < quads) {
                 const int h = tid / (DH / 4), d = tid % (DH / 4) * 4;
                 float4 sum = partial[tid];
+#pragma unroll 1
                 for (int s = 1; s < shares; ++s) {
                     const float4 v = partial[s * quads + tid];
                     sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;

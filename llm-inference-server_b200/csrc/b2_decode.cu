@@ -1586,11 +1586,27 @@ int launch_blocks(K kern, std::atomic<uint64_t>& smem_set, int smem, const P& pr
 // The largest slot is below 2^31, and the chunk index (block, layer, head) too.
 int check_q4_shape(int num_blocks, int n_layer, int n_kv_head, int head_dim) {
     if (head_dim != 64 && head_dim != 128) return fail(B2_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
-    if (num_blocks <= 0 || n_layer <= 0 || n_kv_head <= 0)
-        return fail(B2_ERR_SHAPE, "num_blocks, n_layer and n_kv_head must be positive");
+    if (num_blocks <= 0 || n_layer <= 0 || n_kv_head <= 0 || n_kv_head > 65535)
+        return fail(B2_ERR_SHAPE, "num_blocks and n_layer must be positive, n_kv_head 1 to 65535");
     if (num_blocks > (1 << 27) - 1 || static_cast<double>(num_blocks) * n_layer * n_kv_head >= 2147483648.0)
         return fail(B2_ERR_SHAPE, "num_blocks must stay below 2^27 and num_blocks*n_layer*n_kv_head below 2^31");
     return B2_OK;
+}
+
+// Four rows a CTA once that still gives every SM several CTAs; one below, where the call is
+// latency and more CTAs share it.  Threads: the fewest warps that take the same number of
+// rounds over a row pair's 16-byte pieces as 256 threads would.
+template <typename T, int DH, bool kAppend>
+int launch_kv_q4(const KvQ4Params& p, cudaStream_t s) {
+    int dev = -1;
+    const DeviceInfo di = device_info(&dev);
+    if (dev < 0 || di.sms <= 0) return fail(B2_ERR_DEVICE, "no current CUDA device");
+    const int pieces = 2 * p.n_kv_head * (DH / 8);
+    const int rounds = (pieces + 255) / 256;
+    const dim3 threads(static_cast<unsigned>(((pieces + rounds - 1) / rounds + 31) / 32 * 32));
+    if (p.rows >= 4 * 4 * di.sms)
+        return launch_pdl(kv_q4_kernel<T, DH, kAppend, 4>, dim3(static_cast<unsigned>((p.rows + 3ll) / 4)), threads, 0, s, p);
+    return launch_pdl(kv_q4_kernel<T, DH, kAppend, 1>, dim3(static_cast<unsigned>(p.rows)), threads, 0, s, p);
 }
 
 template <bool kAppend>
@@ -1609,16 +1625,11 @@ int kv_q4(const B2KvQ4Args* a, b2_stream_t stream) {
         return fail(B2_ERR_ALIGN, "pool, k and v must be 16-byte aligned, row_stride a multiple of 8");
     KvQ4Params p{static_cast<uint8_t*>(a->kv_pool), a->k, a->v, a->row_stride, a->slots, a->rows,
                  a->n_kv_head, a->layer_idx, a->n_layer, a->num_blocks};
-    const long long total = 2ll * a->rows * a->n_kv_head * (a->head_dim / 8);
-    const long long grid = (total + 255) / 256;
-    if (grid > 2147483647ll) return fail(B2_ERR_SHAPE, "rows * n_kv_head * head_dim too large for one launch");
-    const dim3 g(static_cast<unsigned>(grid));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a->dtype == B2_F16)
-        return a->head_dim == 64 ? launch_pdl(kv_q4_kernel<__half, 64, kAppend>, g, dim3(256), 0, s, p)
-                                 : launch_pdl(kv_q4_kernel<__half, 128, kAppend>, g, dim3(256), 0, s, p);
-    return a->head_dim == 64 ? launch_pdl(kv_q4_kernel<__nv_bfloat16, 64, kAppend>, g, dim3(256), 0, s, p)
-                             : launch_pdl(kv_q4_kernel<__nv_bfloat16, 128, kAppend>, g, dim3(256), 0, s, p);
+        return a->head_dim == 64 ? launch_kv_q4<__half, 64, kAppend>(p, s) : launch_kv_q4<__half, 128, kAppend>(p, s);
+    return a->head_dim == 64 ? launch_kv_q4<__nv_bfloat16, 64, kAppend>(p, s)
+                             : launch_kv_q4<__nv_bfloat16, 128, kAppend>(p, s);
 }
 
 int check_attn_q4_args(const B2PagedAttnQ4Args* a) {
@@ -1789,6 +1800,10 @@ int b2_paged_attention_q4(const B2PagedAttnQ4Args* a, void* workspace, size_t wo
     p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
     p.softcap = a->softcap;
     p.stages = pl.stages;
+    unsigned up = 0;
+    while ((1ull << up) < static_cast<unsigned long long>(a->n_kv_head)) ++up;
+    p.kv_shift = 31 + up;
+    p.kv_mul = static_cast<unsigned>(((1ull << (31 + up)) + a->n_kv_head - 1) / a->n_kv_head);
     p.stages_log2 = pl.stages == 8 ? 3 : pl.stages == 4 ? 2 : 1;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.ws_count = reinterpret_cast<unsigned*>(ws);

@@ -47,89 +47,131 @@ struct KvQ4Params {
     int rows, n_kv_head, layer_idx, n_layer, num_blocks;
 };
 
-// Four neighbouring lanes share a group, 8 elements (16 bytes) each; a thread
-// handles its 8 elements of K or of V.  Bound: HBM, 2 bytes read and 0.625
-// written an element.
-template <typename T, int DH, bool kAppend>
+// The codes of 8 elements against (m, s), packed from the low nibble up.  With q the fp32
+// product (x - m) * (1 / s), off by at most 2^-22 |q|, rounding q gives the code wherever q is not
+// within 1e-4 of a rounding border; the few elements that are take the division.
+__device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float m, float s) {
+    constexpr float kMagic = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer, ties to even
+    const float rs = __frcp_rn(s);
+    uint32_t codes = 0;
+    float far = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float q = (x[e] - m) * rs;
+        const float k = q + kMagic;
+        far = fmaxf(far, fabsf(q - (k - kMagic)));
+        codes |= static_cast<uint32_t>(min(max(static_cast<int>(__float_as_uint(k) - __float_as_uint(kMagic)), -8), 7) + 8) << (4 * e);
+    }
+    if (far > 0.4999f) {
+        codes = 0;
+#pragma unroll 1
+        for (int e = 7; e >= 0; --e) {
+            float v = x[0];
+#pragma unroll
+            for (int f = 1; f < 8; ++f) v = f == e ? x[f] : v;
+            codes = codes << 4 | static_cast<uint32_t>(fminf(fmaxf(rintf(__fdiv_rn(v - m, s)) + 8.0f, 0.0f), 15.0f));
+        }
+    }
+    return s > 0.0f ? codes : 0x88888888u;
+}
+
+// A CTA takes kRows rows; a thread 8 neighbouring elements (16 bytes) of K or of V in each, four
+// lanes a group of 32.  Bound: HBM, 2 bytes and 0.625 an element.  Several rows a thread keep that many
+// 16-byte loads in flight: at 65536 rows of 8 heads x 128 the read-back took 127 us with one row a thread
+// (and a 64-bit division to find it) and takes KROWS4_GATHER with four.
+template <typename T, int DH, bool kAppend, int kRows>
 __global__ void __launch_bounds__(256) kv_q4_kernel(const KvQ4Params p) {
     using C = Q4Chunk<DH>;
     constexpr int G = C::kGroups;
     pdl_launch_dependents();
     pdl_wait();
-    const int per_row = p.n_kv_head * G * 4;  // threads per K (or V) row
-    const long long idx = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-    // a whole group of four is in or out of range together
-    const long long row2 = idx / per_row;  // row * 2 + (K | V)
-    if (row2 >= 2ll * p.rows) return;
-    const int c = static_cast<int>(idx - row2 * per_row);
-    const long long row = row2 >> 1;
-    const bool is_v = row2 & 1;
-    const int i = c & 3, g = (c >> 2) % G, h = (c >> 2) / G;
-    const int slot = __ldg(p.slots + row);
-    if (slot < 0) return;
-    if (slot / kBlockTokens >= p.num_blocks) {
-        if (c == 0) flag_error(B2_DEVERR_BLOCK_ID);
-        return;
+    const int per_row = p.n_kv_head * G * 4;  // threads for a K (or V) row
+    const long long row0 = static_cast<long long>(blockIdx.x) * kRows;
+    int slot[kRows];
+    unsigned err = 0;
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+        slot[k] = row0 + k < p.rows ? __ldg(p.slots + row0 + k) : -1;
+        if (slot[k] >= 0 && slot[k] / kBlockTokens >= p.num_blocks) {
+            err |= B2_DEVERR_BLOCK_ID;
+            slot[k] = -1;
+        }
     }
-    const int t = slot % kBlockTokens;
-    uint8_t* chunk = p.pool + ((static_cast<size_t>(slot / kBlockTokens) * p.n_layer + p.layer_idx) * p.n_kv_head + h) *
-                                  static_cast<size_t>(C::kBytes);
-    uint32_t* param = reinterpret_cast<uint32_t*>(chunk + (is_v ? C::kVParams : C::kKParams) + C::param(t, g));
-    T* x_at = static_cast<T*>(is_v ? p.v : p.k) + row * p.row_stride + (h * DH + g * 32 + i * 8);
-    uint32_t codes;
-    if (kAppend) {
-        float x[8];
-        unpack16<T>(__ldg(reinterpret_cast<const uint4*>(x_at)), x);
-        bool finite = true;
-        float lo = INFINITY, hi = -INFINITY;
+    if (err != 0 && threadIdx.x == 0) flag_error(err);
+    const size_t block_bytes = static_cast<size_t>(p.n_layer) * p.n_kv_head * C::kBytes;
+#pragma unroll 1
+    for (int c0 = 0; c0 < 2 * per_row; c0 += blockDim.x) {  // whole warps: the shuffles need every lane
+        const int c = c0 + threadIdx.x;
+        const bool mine = c < 2 * per_row;
+        const bool is_v = c >= per_row;
+        const int u = is_v ? c - per_row : c;
+        const int i = u & 3, g = (u >> 2) % G, h = (u >> 2) / G;
+        uint8_t* chunk0 = p.pool + (static_cast<size_t>(p.layer_idx) * p.n_kv_head + h) * C::kBytes;
+        T* x0 = static_cast<T*>(is_v ? p.v : p.k) + row0 * p.row_stride + (h * DH + g * 32 + i * 8);
+        if (kAppend) {
+            uint4 raw[kRows];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            finite = finite && isfinite(x[e]);
-            x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
-            lo = fminf(lo, x[e]);
-            hi = fmaxf(hi, x[e]);
-        }
-        const unsigned mask = 0xfu << (threadIdx.x & 28);
+            for (int k = 0; k < kRows; ++k)
+                raw[k] = mine && slot[k] >= 0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k * p.row_stride)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int d = 1; d < 4; d <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(mask, lo, d));
-            hi = fmaxf(hi, __shfl_xor_sync(mask, hi, d));
-        }
-        finite = __all_sync(mask, finite);
-        const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f));
-        const float s = __half2float(sh);
-        const __half mh = __float2half_rn(fmaf(8.0f, s, lo));
-        const float m = __half2float(mh);
-        codes = 0;
+            for (int k = 0; k < kRows; ++k) {
+                float x[8];
+                unpack16<T>(raw[k], x);
+                float lo = INFINITY, hi = -INFINITY, zero = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float k = s > 0.0f ? rintf(__fdiv_rn(x[e] - m, s)) + 8.0f : 8.0f;
-            codes |= static_cast<uint32_t>(fminf(fmaxf(k, 0.0f), 15.0f)) << (4 * e);
-        }
-        if (!finite) codes = 0x88888888u;
-        if (i == 0)
-            *param = finite ? (static_cast<uint32_t>(__half_as_ushort(sh)) << 16 | __half_as_ushort(mh)) : 0x7fff7fffu;
-        if (!is_v) {
-            *reinterpret_cast<uint32_t*>(chunk + C::k_word(t, i, g)) = codes;
+                for (int e = 0; e < 8; ++e) {
+                    zero = fmaf(x[e], 0.0f, zero);  // NaN if an element is NaN or infinite
+                    x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+                    lo = fminf(lo, x[e]);
+                    hi = fmaxf(hi, x[e]);
+                }
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+                    zero += __shfl_xor_sync(0xffffffffu, zero, d);
+                }
+                const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f));
+                const __half mh = __float2half_rn(fmaf(8.0f, __half2float(sh), lo));
+                if (!mine || slot[k] < 0) continue;
+                const uint32_t codes = q4_codes(x, __half2float(mh), __half2float(sh));
+                const int t = slot[k] % kBlockTokens;
+                uint8_t* chunk = chunk0 + static_cast<size_t>(slot[k] / kBlockTokens) * block_bytes;
+                if (i == 0)
+                    *reinterpret_cast<uint32_t*>(chunk + (is_v ? C::kVParams : C::kKParams) + C::param(t, g)) =
+                        zero == 0.0f ? (static_cast<uint32_t>(__half_as_ushort(sh)) << 16 | __half_as_ushort(mh)) : 0x7fff7fffu;
+                if (!is_v) {
+                    *reinterpret_cast<uint32_t*>(chunk + C::k_word(t, i, g)) = codes;
+                } else {
+                    *reinterpret_cast<uint16_t*>(chunk + C::v_unit(t, 2 * i, g)) = static_cast<uint16_t>(codes);
+                    *reinterpret_cast<uint16_t*>(chunk + C::v_unit(t, 2 * i + 1, g)) = static_cast<uint16_t>(codes >> 16);
+                }
+            }
         } else {
-            *reinterpret_cast<uint16_t*>(chunk + C::v_unit(t, 2 * i, g)) = static_cast<uint16_t>(codes);
-            *reinterpret_cast<uint16_t*>(chunk + C::v_unit(t, 2 * i + 1, g)) = static_cast<uint16_t>(codes >> 16);
-        }
-    } else {
-        const uint32_t w = *param;
-        const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(w >> 16)));
-        const float m = __half2float(__ushort_as_half(static_cast<unsigned short>(w & 0xffffu)));
-        if (!is_v) {
-            codes = *reinterpret_cast<const uint32_t*>(chunk + C::k_word(t, i, g));
-        } else {
-            codes = *reinterpret_cast<const uint16_t*>(chunk + C::v_unit(t, 2 * i, g)) |
-                    static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(chunk + C::v_unit(t, 2 * i + 1, g))) << 16;
-        }
-        float x[8];
+            if (!mine) continue;
+            uint32_t w[kRows], codes[kRows];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            x[e] = fmaf(static_cast<float>(static_cast<int>(codes >> (4 * e) & 15u) - 8), s, m);
-        *reinterpret_cast<uint4*>(x_at) = pack16<T>(x);
+            for (int k = 0; k < kRows; ++k) {
+                if (slot[k] < 0) continue;
+                const int t = slot[k] % kBlockTokens;
+                const uint8_t* chunk = chunk0 + static_cast<size_t>(slot[k] / kBlockTokens) * block_bytes;
+                w[k] = __ldg(reinterpret_cast<const uint32_t*>(chunk + (is_v ? C::kVParams : C::kKParams) + C::param(t, g)));
+                codes[k] = !is_v ? __ldg(reinterpret_cast<const uint32_t*>(chunk + C::k_word(t, i, g)))
+                                 : __ldg(reinterpret_cast<const uint16_t*>(chunk + C::v_unit(t, 2 * i, g))) |
+                                       static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(chunk + C::v_unit(t, 2 * i + 1, g)))) << 16;
+            }
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) {
+                if (slot[k] < 0) continue;
+                const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(w[k] >> 16)));
+                const float m = __half2float(__ushort_as_half(static_cast<unsigned short>(w[k] & 0xffffu)));
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[e] = fmaf(static_cast<float>(static_cast<int>(codes[k] >> (4 * e) & 15u) - 8), s, m);
+                *reinterpret_cast<uint4*>(x0 + k * p.row_stride) = pack16<T>(x);
+            }
+        }
     }
 }
 
