@@ -15,7 +15,9 @@
 //     bits 4-7 give 16 c 2^-24 (subnormals; products with them are exact).  One
 //     AND makes two A-operand elements; no conversion, no bias.
 //   * Scores: A = 16 tokens x 16 dims of K codes, B = the query heads of the kv
-//     head (up to 8 columns).  Per group S += s (A q) + (m - 8 s) sum(q) in fp32.
+//     head (up to 8 columns).  S = sum_g s_g (A q)_g + sum_g (m_g - 8 s_g) Q_g, Q_g the
+//     group's sum of q; the first sum is taken in fp32, the second is one more
+//     product whose columns are m and s and whose B is Q in two f16 parts.
 //     q is scaled by a power of two to at most 2^9, so its f16 form is exact
 //     down to 2^-23 of the row's largest element.
 //   * Values: A = V codes transposed (16 dims x 16 tokens), B = f16(p s 2^k) per
@@ -63,10 +65,11 @@ struct Q4AttnParams {
     float scale, softcap;
 };
 
-constexpr int kQ4Warps = 6;
+constexpr int kQ4Warps = 4;
 constexpr int kQ4Threads = 32 * kQ4Warps;
-constexpr int kQ4CtasPerSm = 2;
+constexpr int q4_ctas_per_sm(int dh) { return dh == 64 ? 4 : 3; }
 constexpr int kQ4MaxGroup = 8;
+constexpr int kQ4FewParts = 4;  // parts of an item that a CTA merges straight from L2
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Bytes of one piece's state in shared memory: [group][head_dim] sums, [group] (R, l).
@@ -142,7 +145,7 @@ struct Q4State {
     int k;
     uint32_t s_limit;    // param words from here on need a smaller k
     uint32_t qf[G][4];   // B fragments of head r
-    float qs[G][2];      // 2^-24 sum of q over the group, heads 2i, 2i+1
+    uint32_t qb[2];      // B fragment of head r: Q_i 2^-6 as (high, low) f16 parts, and -8 times them
     float sc[2];         // S -> score (log2 units; with a cap: the exponent's argument)
     float slope[2];      // log2 units
 };
@@ -174,29 +177,31 @@ __device__ __forceinline__ void q4_start(const Q4AttnParams& p, int b, int hk, Q
     const int e2 = static_cast<int>(__float_as_uint(top) >> 23);  // biased exponent, 255 for an infinity
     const int up = e2 == 255 ? 0 : min(135 - e2, 126);
     const float norm = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-    float qsum[G];
+    float sum_i = 0.0f;  // Q_i = sum of q over group i
 #pragma unroll
     for (int g = 0; g < G; ++g) {
         const float f16th = norm * 0.0625f;
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(x[g][e], norm, sum);
         st.qf[g][0] = half2_bits(x[g][0] * norm, x[g][4] * norm);
         st.qf[g][1] = half2_bits(x[g][1] * f16th, x[g][5] * f16th);
         st.qf[g][2] = half2_bits(x[g][2] * norm, x[g][6] * norm);
         st.qf[g][3] = half2_bits(x[g][3] * f16th, x[g][7] * f16th);
-        const float2 a = half2_floats(st.qf[g][0]), c = half2_floats(st.qf[g][1]);
-        const float2 d = half2_floats(st.qf[g][2]), f = half2_floats(st.qf[g][3]);
-        float sum = (a.x + a.y) + (d.x + d.y) + 16.0f * ((c.x + c.y) + (f.x + f.y));
 #pragma unroll
         for (int s = 1; s < 4; s <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-        qsum[g] = sum * 0x1p-24f;
+        if (g == i) sum_i = sum;
     }
+    sum_i *= 0x1p-6f;
+    const float high = __half2float(__float2half_rn(sum_i));
+    st.qb[0] = half2_bits(high, sum_i - high);
+    st.qb[1] = half2_bits(-8.0f * high, -8.0f * (sum_i - high));
     // score = S 2^24 / norm * scale; the cap's argument is 2 score / cap (exp of it in log2 units)
     const float unit = p.softcap > 0.0f ? 2.0f * kLog2e * p.scale / p.softcap : kLog2e * p.scale;
     const float sc = unit * 0x1p24f * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int src = 4 * (2 * i + h);
-#pragma unroll
-        for (int g = 0; g < G; ++g) st.qs[g][h] = __shfl_sync(0xffffffffu, qsum[g], src);
         st.sc[h] = __shfl_sync(0xffffffffu, sc, src);
         st.slope[h] = p.slopes != nullptr && 2 * i + h < p.group ? __ldg(p.slopes + hk * p.group + 2 * i + h) * kLog2e : 0.0f;
         st.ref[h] = -FLT_MAX;
@@ -220,13 +225,14 @@ struct Q4Lane {
     // later).  Chosen so that the rows' K words, the lanes' V words and all params are read
     // without bank conflicts.
     int tk;
-    uint32_t k, kp, va, vb, ma, mb;
+    uint32_t k, kp, kpi, va, vb, ma, mb;
     __device__ __forceinline__ Q4Lane() {
         const int lane = threadIdx.x & 31, r = lane >> 2, i = lane & 3;
         tk = (r & 1) ? 4 + ((r >> 1) ^ 3) : r >> 1;
         const int ta = i, tb = 4 + (i ^ 3);
         k = C::k_word(tk, i, 0);
         kp = C::kKParams + C::param(tk, 0);
+        kpi = C::kKParams + C::param(tk, i & (C::kGroups - 1));
         va = C::v_unit(ta, r, 0);
         vb = C::v_unit(tb, r, 0);
         ma = C::kVParams + C::param(ta, r & (C::kGroups - 1));
@@ -267,22 +273,32 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
         ld_words<G>(stage[u] + at.k + 8 * (DH / 2), kb);
         ld_words<G>(stage[u] + at.kp, pa);
         ld_words<G>(stage[u] + at.kp + 8 * 4 * G, pb);
-        x[2 * u][0] = x[2 * u][1] = x[2 * u + 1][0] = x[2 * u + 1][1] = 0.0f;
+        // sum over the groups of (m - 8 s) Q_g: columns (m_i, m_i, s_i, s_i) against (Q_i, -8 Q_i)
+        float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        {
+            const uint32_t wa = ld_word(stage[u] + at.kpi), wb = ld_word(stage[u] + at.kpi + 8 * 4 * G);
+            mma_f16(z, __byte_perm(wa, wa, 0x1010), __byte_perm(wb, wb, 0x1010), __byte_perm(wa, wa, 0x3232),
+                    __byte_perm(wb, wb, 0x3232), st.qb[0], st.qb[1]);
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[2 * u + t][h] = z[2 * t + h] * 0x1p-18f;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             mma_f16(c, ka[g] & kLow, kb[g] & kLow, ka[g] & kHigh, kb[g] & kHigh, st.qf[g][0], st.qf[g][1]);
             const uint32_t ua = ka[g] >> 8, ub = kb[g] >> 8;
             mma_f16(c, ua & kLow, ub & kLow, ua & kHigh, ub & kHigh, st.qf[g][2], st.qf[g][3]);
-            const float2 a = half2_floats(pa[g]), b = half2_floats(pb[g]);  // (m, s)
-            const float ma = fmaf(-8.0f, a.y, a.x), mb = fmaf(-8.0f, b.y, b.x);
+            const float sa = half2_floats(pa[g]).y, sb = half2_floats(pb[g]).y;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                x[2 * u][h] = fmaf(a.y, c[h], fmaf(ma, st.qs[g][h], x[2 * u][h]));
-                x[2 * u + 1][h] = fmaf(b.y, c[2 + h], fmaf(mb, st.qs[g][h], x[2 * u + 1][h]));
+                x[2 * u][h] = fmaf(sa, c[h], x[2 * u][h]);
+                x[2 * u + 1][h] = fmaf(sb, c[2 + h], x[2 * u + 1][h]);
             }
         }
     }
+    // Rounded before the reference is taken off: the largest score's weight is 1 however large it is.
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -434,7 +450,7 @@ struct Q4Entry {
 
 // Dynamic shared memory: [warp][stages] chunks, [warp] first pieces, [warp][stages] barriers.
 template <typename T, typename OutT, int DH>
-__global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kernel(const Q4AttnParams p) {
+__global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q4_kernel(const Q4AttnParams p) {
     using C = Q4Chunk<DH>;
     constexpr int G = DH / 32;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -531,7 +547,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 if (2 * i + h < p.group) {
-                    const float inv = 1.0f / l[h];
+                    const float inv = __fdividef(1.0f, l[h]);
                     OutT* row = static_cast<OutT*>(p.out) +
                                 (static_cast<size_t>(b) * p.n_head + hk * p.group + 2 * i + h) * DH + 4 * r;
 #pragma unroll
@@ -667,7 +683,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
             }
             if (en.start >= cta0 && en.start + en.count <= cta1) {
                 const int b = q4_sequence(p, en.item), hk = en.item - b * p.n_kv_head;
-                const float inv = 1.0f / l;
+                const float inv = __fdividef(1.0f, l);
                 OutT* row = static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH;
 #pragma unroll
                 for (int g = 0; g < G; ++g) row[32 * g + lane] = Elem<OutT>::from_f(sum[g] * inv);
@@ -713,6 +729,40 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
         const int b = q4_sequence(p, en.item), hk = en.item - b * p.n_kv_head;
         // workspace row of part j and head h: the item's first CTA wrote its slot 1, the others slot 0
         auto row_of = [&](int j, int h) { return (2 * (f + j) + (j == 0 ? 1 : 0)) * p.group + h; };
+        if (parts_n <= kQ4FewParts) {  // the usual case, in one trip to L2: every thread reads all it needs at once
+#pragma unroll 1
+            for (int e = tid * 4; e < p.group * DH; e += kQ4Threads * 4) {
+                const int h = e / DH, d = e % DH;
+                float2 ml[kQ4FewParts];
+                float4 v[kQ4FewParts];
+#pragma unroll
+                for (int j = 0; j < kQ4FewParts; ++j) {
+                    ml[j] = make_float2(-FLT_MAX, 0.0f);
+                    v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (j < parts_n) {
+                        ml[j] = __ldcg(p.ws_ml + row_of(j, h));
+                        v[j] = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + static_cast<size_t>(row_of(j, h)) * DH + d));
+                    }
+                }
+                float top = ml[0].x, l = 0.0f;
+#pragma unroll
+                for (int j = 1; j < kQ4FewParts; ++j) top = fmaxf(top, ml[j].x);
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int j = 0; j < kQ4FewParts; ++j) {
+                    const float w = ex2_approx(ml[j].x - top);
+                    l = fmaf(ml[j].y, w, l);
+                    sum.x = fmaf(v[j].x, w, sum.x);
+                    sum.y = fmaf(v[j].y, w, sum.y);
+                    sum.z = fmaf(v[j].z, w, sum.z);
+                    sum.w = fmaf(v[j].w, w, sum.w);
+                }
+                const float inv = __fdividef(1.0f, l);
+                q4_store4<OutT>(static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH + d,
+                                sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            }
+            continue;
+        }
         // the parts' weights and l, per head, in the (drained) rings: [group][parts] and [group]
         float* weight = reinterpret_cast<float*>(smem);
         float* denom = weight + p.group * parts_n;
@@ -762,7 +812,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
             if (shares > 1) {
                 partial[e] = sum;
             } else {
-                const float inv = 1.0f / denom[h];
+                const float inv = __fdividef(1.0f, denom[h]);
                 q4_store4<OutT>(static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH + d,
                                 sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
             }
@@ -777,7 +827,7 @@ __global__ void __launch_bounds__(kQ4Threads, kQ4CtasPerSm) paged_decode_q4_kern
                     const float4 v = partial[s * quads + tid];
                     sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
                 }
-                const float inv = 1.0f / denom[h];
+                const float inv = __fdividef(1.0f, denom[h]);
                 q4_store4<OutT>(static_cast<OutT*>(p.out) + (static_cast<size_t>(b) * p.n_head + hk * p.group + h) * DH + d,
                                 sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
             }

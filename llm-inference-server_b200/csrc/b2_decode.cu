@@ -1667,22 +1667,22 @@ struct Q4Plan {
     size_t ws_count = 0, ws_ml = 0, ws_total = 0;  // [counters][(R, l)][sums]
 };
 
-// Two CTAs per SM; as many ring stages (2, 4 or 8) as their half of the shared memory holds.
+// As many ring stages (2, 4 or 8) as a CTA's share of its SM's shared memory holds.
 int plan_attn_q4(const B2PagedAttnQ4Args* a, Q4Plan* pl) {
     int dev = -1;
     const DeviceInfo di = device_info(&dev);
     if (dev < 0 || di.sms <= 0) return fail(B2_ERR_DEVICE, "no current CUDA device");
-    const int group = a->n_head / a->n_kv_head;
+    const int group = a->n_head / a->n_kv_head, per_sm = q4_ctas_per_sm(a->head_dim);
     const int pieces = kQ4Warps * q4_piece_bytes(group, a->head_dim);
     const int per_stage = kQ4Warps * (20 * a->head_dim + 8);
-    const int room = di.smem_per_sm / kQ4CtasPerSm - 1024 - 2048;  // reserved and static shared memory
+    const int room = di.smem_per_sm / per_sm - 1024 - 1536;  // reserved and static shared memory
     const int fit = (room - pieces) / per_stage;
     pl->stages = fit >= 8 ? 8 : fit >= 4 ? 4 : fit >= 2 ? 2 : 0;
     // a warp's last piece is kept in its drained ring
     if (pl->stages < 2 || pl->stages * 20 * a->head_dim < q4_piece_bytes(group, a->head_dim))
         return fail(B2_ERR_UNSUPPORTED, "4-bit attention: shared memory");
     pl->smem = pieces + pl->stages * per_stage;
-    pl->grid = di.sms * kQ4CtasPerSm;
+    pl->grid = di.sms * per_sm;
     if (a->max_ctas > 0) pl->grid = std::min(pl->grid, a->max_ctas);
     const size_t slots = 2 * static_cast<size_t>(pl->grid) * group;
     pl->ws_count = align_up(static_cast<size_t>(pl->grid) * sizeof(unsigned), 256);
@@ -1697,7 +1697,7 @@ int launch_attn_q4_t(const Q4Plan& pl, const Q4AttnParams& p, cudaStream_t s) {
     static std::atomic<uint64_t> smem_set{0};
     int dev = -1;
     const DeviceInfo di = device_info(&dev);
-    const int rc = ensure_max_smem(kern, smem_set, dev, di.smem_per_sm / kQ4CtasPerSm - 1024 - 2048);
+    const int rc = ensure_max_smem(kern, smem_set, dev, di.smem_per_sm / q4_ctas_per_sm(DH) - 1024 - 1536);
     if (rc != B2_OK) return rc;
     return launch_pdl(kern, dim3(static_cast<unsigned>(pl.grid)), dim3(kQ4Threads), pl.smem, s, p);
 }
