@@ -60,7 +60,6 @@ struct Q4AttnParams {
     float2* ws_ml;       // [2 grid][group]
     float* ws_acc;       // [2 grid][group][head_dim]
     int batch, n_head, n_kv_head, group, mbps, layer_idx, n_layer, num_blocks, window;
-    int stages, stages_log2;
     unsigned kv_mul, kv_shift;  // n / n_kv_head = n * kv_mul >> kv_shift for n < 2^31
     float scale, softcap;
 };
@@ -68,6 +67,7 @@ struct Q4AttnParams {
 constexpr int kQ4Warps = 4;
 constexpr int kQ4Threads = 32 * kQ4Warps;
 constexpr int q4_ctas_per_sm(int dh) { return dh == 64 ? 4 : 3; }
+constexpr int kQ4Slots = 2;  // ring slots of a warp, a step (two chunks) each
 constexpr int kQ4MaxGroup = 8;
 constexpr int kQ4FewParts = 4;  // parts of an item that a CTA merges straight from L2
 constexpr float kLog2e = 1.4426950408889634f;
@@ -93,9 +93,9 @@ __device__ __forceinline__ int q4_sequence(const Q4AttnParams& p, int item) {
     return static_cast<int>(static_cast<unsigned long long>(static_cast<unsigned>(item)) * p.kv_mul >> p.kv_shift);
 }
 
-// Blocks that hold visible keys.
-__device__ __forceinline__ int q4_blocks(int first, int n) {
-    return first < n ? (n - 1) / kBlockTokens - first / kBlockTokens + 1 : 0;
+// Steps (two blocks, the last one maybe one) over the blocks that hold visible keys.
+__device__ __forceinline__ int q4_steps(int first, int n) {
+    return first < n ? ((n - 1) / kBlockTokens - first / kBlockTokens) / 2 + 1 : 0;
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -105,6 +105,13 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The product alone (C = 0).
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -240,13 +247,13 @@ struct Q4Lane {
     }
 };
 
-// Two chunks of 16 tokens at shared addresses stage[0] and stage[1], positions blk * 16 on and 16
-// later, keys [first, n) visible.  Two at a time: their products are independent, and the
-// softmax's bookkeeping is paid once.  Where the warp has only one chunk left, stage[1] is stage[0]
-// and n ends at the first chunk: a masked token's weight is 0, its codes and steps are finite.
+// One step: two chunks of 16 tokens at shared addresses stage[0] and stage[1], positions blk * 16 on
+// and 16 later, keys [first, n) visible.  Two at a time: their products are independent, and the
+// bookkeeping is paid once.  Where the item ends with the first chunk, stage[1] is stage[0]: the second
+// chunk's tokens are past n, so their weights are 0, and the steps and middles that those meet are the first one's.
 template <int DH>
 __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>& at, const uint32_t (&stage)[2], int blk,
-                                        int first, int n, int last, Q4State<DH>& st) {
+                                        int first, int n, Q4State<DH>& st) {
     using C = Q4Chunk<DH>;
     constexpr int G = DH / 32;
     constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
@@ -274,27 +281,33 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
         ld_words<G>(stage[u] + at.kp, pa);
         ld_words<G>(stage[u] + at.kp + 8 * 4 * G, pb);
         // sum over the groups of (m - 8 s) Q_g: columns (m_i, m_i, s_i, s_i) against (Q_i, -8 Q_i)
-        float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float z[4];
         {
             const uint32_t wa = ld_word(stage[u] + at.kpi), wb = ld_word(stage[u] + at.kpi + 8 * 4 * G);
-            mma_f16(z, __byte_perm(wa, wa, 0x1010), __byte_perm(wb, wb, 0x1010), __byte_perm(wa, wa, 0x3232),
+            mma_f16_first(z, __byte_perm(wa, wa, 0x1010), __byte_perm(wb, wb, 0x1010), __byte_perm(wa, wa, 0x3232),
                     __byte_perm(wb, wb, 0x3232), st.qb[0], st.qb[1]);
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int h = 0; h < 2; ++h) x[2 * u + t][h] = z[2 * t + h] * 0x1p-18f;
+        // A product that adds to another's sum waits for it (some 20 cycles): all first ones go before all second ones.
+        float c[G][4];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+            mma_f16_first(c[g], ka[g] & kLow, kb[g] & kLow, ka[g] & kHigh, kb[g] & kHigh, st.qf[g][0], st.qf[g][1]);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma_f16(c, ka[g] & kLow, kb[g] & kLow, ka[g] & kHigh, kb[g] & kHigh, st.qf[g][0], st.qf[g][1]);
             const uint32_t ua = ka[g] >> 8, ub = kb[g] >> 8;
-            mma_f16(c, ua & kLow, ub & kLow, ua & kHigh, ub & kHigh, st.qf[g][2], st.qf[g][3]);
+            mma_f16(c[g], ua & kLow, ub & kLow, ua & kHigh, ub & kHigh, st.qf[g][2], st.qf[g][3]);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
             const float sa = half2_floats(pa[g]).y, sb = half2_floats(pb[g]).y;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                x[2 * u][h] = fmaf(sa, c[h], x[2 * u][h]);
-                x[2 * u + 1][h] = fmaf(sb, c[2 + h], x[2 * u + 1][h]);
+                x[2 * u][h] = fmaf(sa, c[g][h], x[2 * u][h]);
+                x[2 * u + 1][h] = fmaf(sb, c[g][2 + h], x[2 * u + 1][h]);
             }
         }
     }
@@ -312,7 +325,7 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
                 x[t][h] = cap - __fdividef(2.0f * cap, 1.0f + ex2_approx(x[t][h]));
     }
     if (p.slopes != nullptr) {
-        const float d = static_cast<float>(pos + at.tk - last);
+        const float d = static_cast<float>(pos + at.tk - (n - 1));
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -393,19 +406,26 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
         ld_words<G / 2>(stage[u] + at.vb, v[1]);
         ld_words<G / 2>(stage[u] + at.va + 256, v[2]);
         ld_words<G / 2>(stage[u] + at.vb + 256, v[3]);
+        uint32_t b0[G], b1[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const float sa = half2_floats(vp[2 * u][g]).y, sb = half2_floats(vp[2 * u + 1][g]).y;
-            const uint32_t b0 = transpose8x8(half2_bits(x[2 * u][0] * sa, x[2 * u][1] * sa));
-            const uint32_t b1 = transpose8x8(half2_bits(x[2 * u + 1][0] * sb, x[2 * u + 1][1] * sb));
+            b0[g] = transpose8x8(half2_bits(x[2 * u][0] * sa, x[2 * u][1] * sa));
+            b1[g] = transpose8x8(half2_bits(x[2 * u + 1][0] * sb, x[2 * u + 1][1] * sb));
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
             const uint32_t pick = g & 1 ? 0x7632 : 0x5410;
             const uint32_t u0 = __byte_perm(v[0][g / 2], v[1][g / 2], pick), u1 = __byte_perm(v[2][g / 2], v[3][g / 2], pick);
-            mma_f16(st.acc[g][0], u0 & kLow, u0 & kHigh, u1 & kLow, u1 & kHigh, b0, b1);
+            mma_f16(st.acc[g][0], u0 & kLow, u0 & kHigh, u1 & kLow, u1 & kHigh, b0[g], b1[g]);
             const uint32_t w0 = u0 >> 8, w1 = u1 >> 8;
-            mma_f16(st.acc[g][1], w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh, b0, b1);
-            // -8 in the units of even and odd dims: -8 2^-24 and -8 16 2^-24
-            mma_f16(st.acc[g][0], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
-            mma_f16(st.acc[g][1], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);
+            mma_f16(st.acc[g][1], w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh, b0[g], b1[g]);
+        }
+        // -8 in the units of even and odd dims: -8 2^-24 and -8 16 2^-24
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            mma_f16(st.acc[g][0], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0[g], b1[g]);
+            mma_f16(st.acc[g][1], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0[g], b1[g]);
         }
     }
 }
@@ -444,11 +464,11 @@ __device__ __forceinline__ void q4_store4(OutT* at, float a, float b, float c, f
 
 struct Q4Entry {
     int item;        // -1: none
-    unsigned start;  // the item's first chunk in the list
-    unsigned count;  // its chunks
+    unsigned start;  // the item's first step in the list
+    unsigned count;  // its steps
 };
 
-// Dynamic shared memory: [warp][stages] chunks, [warp] first pieces, [warp][stages] barriers.
+// Dynamic shared memory: [warp][slot] steps of two chunks, [warp] first pieces.
 template <typename T, typename OutT, int DH>
 __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q4_kernel(const Q4AttnParams p) {
     using C = Q4Chunk<DH>;
@@ -460,18 +480,21 @@ __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q
     __shared__ int s_last[2];
     __shared__ int2 s_parts[2];  // their first CTA and number of CTAs
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane & 3, r = lane >> 2;
+    __shared__ uint64_t s_bars[kQ4Warps][kQ4Slots];
+    __shared__ int4 s_list[kQ4Warps][64];  // the warp's next steps: (chunk, chunk or -1, item, first block)
     const int piece_bytes = q4_piece_bytes(p.group, DH);
-    uint8_t* ring = smem + static_cast<size_t>(warp) * p.stages * C::kBytes;
-    uint8_t* pieces = smem + static_cast<size_t>(kQ4Warps) * p.stages * C::kBytes;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(pieces + kQ4Warps * piece_bytes) + warp * p.stages;
+    constexpr int kRing = kQ4Slots * 2 * C::kBytes;
+    uint8_t* ring = smem + warp * kRing;
+    uint8_t* pieces = smem + kQ4Warps * kRing;
+    uint64_t* bars = s_bars[warp];
     // A piece's state: slot 0 (the warp's first chunks) has its own room, slot 1 (its last) takes the drained ring.
     auto piece_at = [&](int w, int slot) {
         return reinterpret_cast<float*>(slot == 0 ? pieces + w * piece_bytes
-                                                  : smem + static_cast<size_t>(w) * p.stages * C::kBytes);
+                                                  : smem + w * kRing);
     };
     if (lane == 0) {
 #pragma unroll 1
-        for (int s = 0; s < p.stages; ++s) mbar_init(bars + s, 1);
+        for (int s = 0; s < kQ4Slots; ++s) mbar_init(bars + s, 1);
         fence_mbar_init();
     }
     if (tid < 2 * kQ4Warps) s_entry[tid].item = -1;
@@ -479,7 +502,7 @@ __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q
     pdl_launch_dependents();
     pdl_wait();
 
-    // The list: chunks before each thread's share of the sequences.
+    // The list of steps, by sequence, kv head and block: how many come before each thread's share of the sequences.
     unsigned err = 0;
     const int per = (p.batch + kQ4Threads - 1) / kQ4Threads;
     unsigned mine = 0;
@@ -487,51 +510,57 @@ __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q
     for (int b = min(tid * per, p.batch); b < min((tid + 1) * per, p.batch); ++b) {
         int first, n;
         q4_range(p, b, &first, &n, &err);
-        mine += static_cast<unsigned>(q4_blocks(first, n)) * p.n_kv_head;
+        mine += static_cast<unsigned>(q4_steps(first, n)) * p.n_kv_head;
     }
     if (blockIdx.x != 0) err = 0;
     unsigned total;
     s_seg[tid] = block_scan(mine, 0x7fffffffu, s_scan, &total);
     __syncthreads();
-    // Fewer CTAs than launched where a warp would get less than a chunk.
+    // Fewer CTAs than launched where a warp would get less than a step.
     const unsigned ctas = max(1u, min(gridDim.x, (total + kQ4Warps - 1) / kQ4Warps));
-    // Part (warp) i of the list: `each` chunks, one more for the first `more` parts.
+    // Part (warp) i of the list: `each` steps, one more for the first `more` parts.
     const unsigned parts = ctas * kQ4Warps, each = total / parts, more = total - each * parts;
     auto bound = [&](unsigned part) { return part * each + min(part, more); };
     const bool active = blockIdx.x < ctas;
     const unsigned c0 = active ? bound(blockIdx.x * kQ4Warps + warp) : 0;
     const unsigned c1 = active ? bound(blockIdx.x * kQ4Warps + warp + 1) : 0;
 
-    // Lane's chunk of the 32 from `from` on: where it lies and what it is.
-    auto locate = [&](unsigned from, unsigned* chunk, int* item, int* blk) {
-        const unsigned c = from + lane;
-        if (c >= c1) return;
-        const int seg = last_at_most(s_seg, kQ4Threads, c);
-        unsigned base = s_seg[seg];
-        int b = seg * per, first, n, nb;
-        unsigned none = 0;
+    // Puts the 32 steps from `at` on into the warp's list, a step to a lane.
+    auto locate = [&](unsigned at) {
+        const unsigned c = at + lane;
+        if (c < c1) {
+            const int seg = last_at_most(s_seg, kQ4Threads, c);
+            unsigned base = s_seg[seg];
+            int b = seg * per, first, n, steps;
+            unsigned none = 0;
 #pragma unroll 1
-        for (;; ++b) {
-            q4_range(p, b, &first, &n, &none);
-            nb = q4_blocks(first, n);
-            if (c < base + static_cast<unsigned>(nb) * p.n_kv_head || b + 1 == p.batch) break;
-            base += static_cast<unsigned>(nb) * p.n_kv_head;
+            for (;; ++b) {
+                q4_range(p, b, &first, &n, &none);
+                steps = q4_steps(first, n);
+                if (c < base + static_cast<unsigned>(steps) * p.n_kv_head || b + 1 == p.batch) break;
+                base += static_cast<unsigned>(steps) * p.n_kv_head;
+            }
+            const int h = static_cast<int>(c - base) / steps;
+            const int blk = first / kBlockTokens + 2 * (static_cast<int>(c - base) - h * steps);
+            const int* entry = p.block_tables + static_cast<size_t>(b) * p.mbps + blk;
+            const bool two = (blk + 1) * kBlockTokens < n;
+            int id[2] = {__ldg(entry), two ? __ldg(entry + 1) : 0};
+            int4 step = make_int4(0, -1, b * p.n_kv_head + h, blk);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (id[k] < 0 || id[k] >= p.num_blocks) {
+                    err |= B2_DEVERR_BLOCK_ID;
+                    id[k] = min(max(id[k], 0), p.num_blocks - 1);
+                }
+                id[k] = static_cast<int>((static_cast<long long>(id[k]) * p.n_layer + p.layer_idx) * p.n_kv_head + h);
+            }
+            step.x = id[0];
+            if (two) step.y = id[1];
+            s_list[warp][c & 63] = step;
         }
-        const int h = static_cast<int>(c - base) / nb;
-        *blk = first / kBlockTokens + static_cast<int>(c - base) - h * nb;
-        *item = b * p.n_kv_head + h;
-        int id = __ldg(p.block_tables + static_cast<size_t>(b) * p.mbps + *blk);
-        if (id < 0 || id >= p.num_blocks) {
-            err |= B2_DEVERR_BLOCK_ID;
-            id = min(max(id, 0), p.num_blocks - 1);
-        }
-        *chunk = static_cast<unsigned>((static_cast<long long>(id) * p.n_layer + p.layer_idx) * p.n_kv_head + h);
+        __syncwarp();
     };
-    // Two windows of 32 chunks, a chunk to a lane: the one from window_at on and the one before it.
-    unsigned new_chunk = 0, old_chunk = 0;
-    int new_item = -1, new_blk = 0, old_item = -1, old_blk = 0;
-    unsigned window_at = c0 - 32, issued = c0;
-    const unsigned slot_mask = p.stages - 1;
+    unsigned located = c0, issued = c0;
     const uint32_t ring_at = smem_addr(ring);
 
     Q4State<DH> st;
@@ -542,8 +571,8 @@ __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q
         float o[2][G][4], l[2];
         q4_finish<DH>(st, o, l);
         const int b = q4_sequence(p, item), hk = item - b * p.n_kv_head;
-        const int nb = q4_blocks(first, n);
-        if (upto - from == static_cast<unsigned>(nb)) {
+        const int steps = q4_steps(first, n);
+        if (upto - from == static_cast<unsigned>(steps)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 if (2 * i + h < p.group) {
@@ -568,64 +597,58 @@ __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q
                 if (r == 0) *reinterpret_cast<float2*>(at + p.group * DH + 2 * (2 * i + h)) = make_float2(st.ref[h], l[h]);
             }
         if (lane == 0)
-            s_entry[2 * warp + slot] = Q4Entry{item, from - static_cast<unsigned>(from_blk - first / kBlockTokens),
-                                               static_cast<unsigned>(nb)};
+            s_entry[2 * warp + slot] = Q4Entry{item, from - static_cast<unsigned>((from_blk - first / kBlockTokens) / 2),
+                                               static_cast<unsigned>(steps)};
     };
     const Q4Lane<DH> offs;
     bool alive = true;
     unsigned c = c0, item_end = c0;
     int blk = 0;
     while (c0 < c1) {
-        // Refill the ring: a lane copies its own chunk where that is among the next ones to copy.
-        const unsigned limit = min(c1, c + p.stages);
-        if (limit > window_at + 32) {
-            old_chunk = new_chunk, old_item = new_item, old_blk = new_blk;
-            window_at += 32;
-            locate(window_at, &new_chunk, &new_item, &new_blk);
+        // Refill the ring: a lane copies a step.
+        const unsigned limit = min(c1, c + kQ4Slots);
+        if (limit > located) {
+            locate(located);
+            located += 32;
         }
-        {
-            const bool in_new = window_at + lane < limit;
-            const unsigned idx = in_new ? window_at + lane : window_at + lane - 32;
-            if (static_cast<int>(idx - issued) >= 0 && idx < limit) {
-                const unsigned slot = (idx - c0) & slot_mask;
-                mbar_arrive_expect_tx(bars + slot, C::kBytes);
-                bulk_g2s(ring + slot * C::kBytes,
-                         p.pool + static_cast<size_t>(in_new ? new_chunk : old_chunk) * C::kBytes, C::kBytes, bars + slot);
-            }
-            issued = limit;
-            __syncwarp();
+        if (issued + lane < limit) {
+            const unsigned idx = issued + lane, slot = (idx - c0) % kQ4Slots;
+            const int4 step = s_list[warp][idx & 63];
+            mbar_arrive_expect_tx(bars + slot, step.y >= 0 ? 2 * C::kBytes : C::kBytes);
+            uint8_t* to = ring + slot * 2 * C::kBytes;
+            bulk_g2s(to, p.pool + static_cast<size_t>(step.x) * C::kBytes, C::kBytes, bars + slot);
+            if (step.y >= 0)
+                bulk_g2s(to + C::kBytes, p.pool + static_cast<size_t>(step.y) * C::kBytes, C::kBytes, bars + slot);
         }
+        issued = limit;
+        __syncwarp();
         if (c == item_end) {
             if (item >= 0) end_item(c);
             if (c == c1) break;
-            const bool in_new = static_cast<int>(c - window_at) >= 0;
-            const int src = static_cast<int>((c - c0) & 31);
-            item = __shfl_sync(0xffffffffu, in_new ? new_item : old_item, src);
-            blk = __shfl_sync(0xffffffffu, in_new ? new_blk : old_blk, src);
+            const int4 step = s_list[warp][c & 63];
+            item = step.z;
             from = c;
-            from_blk = blk;
+            from_blk = blk = step.w;
             const int b = q4_sequence(p, item);
             unsigned none = 0;
             q4_range(p, b, &first, &n, &none);
-            item_end = min(c1, c + static_cast<unsigned>((n - 1) / kBlockTokens - blk + 1));
+            item_end = min(c1, c + static_cast<unsigned>(((n - 1) / kBlockTokens - blk) / 2 + 1));
             q4_start<T, DH>(p, b, item - b * p.n_kv_head, st);
         }
-        const bool two = c + 1 < item_end;
-        const unsigned k0 = c - c0, k1 = two ? k0 + 1 : k0;
-        const unsigned s0 = k0 & slot_mask, s1 = k1 & slot_mask;
-        alive = __all_sync(0xffffffffu, mbar_wait_bounded(bars + s0, (k0 >> p.stages_log2) & 1) &&
-                                            mbar_wait_bounded(bars + s1, (k1 >> p.stages_log2) & 1));
+        const unsigned slot = (c - c0) % kQ4Slots;
+        alive = __all_sync(0xffffffffu, mbar_wait_bounded(bars + slot, (c - c0) / kQ4Slots & 1));
         if (!alive) break;
-        const uint32_t at[2] = {ring_at + s0 * C::kBytes, ring_at + s1 * C::kBytes};
-        q4_step<DH>(p, offs, at, blk, first, two ? n : min(n, (blk + 1) * kBlockTokens), n - 1, st);
-        __syncwarp();  // every lane is done with the slots
-        c += two ? 2 : 1;
-        blk += two ? 2 : 1;
+        const uint32_t first_at = ring_at + slot * 2 * C::kBytes;
+        const uint32_t at[2] = {first_at, (blk + 1) * kBlockTokens < n ? first_at + C::kBytes : first_at};
+        q4_step<DH>(p, offs, at, blk, first, n, st);
+        __syncwarp();  // every lane is done with the slot
+        ++c;
+        blk += 2;
     }
     if (!alive) {  // the copies in flight end before this CTA's shared memory goes
         err |= B2_DEVERR_TIMEOUT;
 #pragma unroll 1
-        for (; c < issued; ++c) mbar_wait_bounded(bars + ((c - c0) & slot_mask), ((c - c0) >> p.stages_log2) & 1);
+        for (; c < issued; ++c) mbar_wait_bounded(bars + (c - c0) % kQ4Slots, (c - c0) / kQ4Slots & 1);
     }
     // Sequences without a visible key.
 #pragma unroll 1

@@ -1662,28 +1662,29 @@ int check_attn_q4_args(const B2PagedAttnQ4Args* a) {
     return B2_OK;
 }
 
+// A CTA's share of its SM's shared memory, less what is reserved and the kernel's static arrays.
+int q4_max_smem(const DeviceInfo& di, int head_dim) { return di.smem_per_sm / q4_ctas_per_sm(head_dim) - 1024 - 6144; }
+
 struct Q4Plan {
-    int grid = 0, stages = 0, smem = 0;
+    int grid = 0, smem = 0;
     size_t ws_count = 0, ws_ml = 0, ws_total = 0;  // [counters][(R, l)][sums]
 };
 
-// As many ring stages (2, 4 or 8) as a CTA's share of its SM's shared memory holds.
 int plan_attn_q4(const B2PagedAttnQ4Args* a, Q4Plan* pl) {
     int dev = -1;
     const DeviceInfo di = device_info(&dev);
     if (dev < 0 || di.sms <= 0) return fail(B2_ERR_DEVICE, "no current CUDA device");
     const int group = a->n_head / a->n_kv_head, per_sm = q4_ctas_per_sm(a->head_dim);
     const int pieces = kQ4Warps * q4_piece_bytes(group, a->head_dim);
-    const int per_stage = kQ4Warps * (20 * a->head_dim + 8);
-    const int room = di.smem_per_sm / per_sm - 1024 - 1536;  // reserved and static shared memory
-    const int fit = (room - pieces) / per_stage;
-    pl->stages = fit >= 8 ? 8 : fit >= 4 ? 4 : fit >= 2 ? 2 : 0;
-    // a warp's last piece is kept in its drained ring
-    if (pl->stages < 2 || pl->stages * 20 * a->head_dim < q4_piece_bytes(group, a->head_dim))
-        return fail(B2_ERR_UNSUPPORTED, "4-bit attention: shared memory");
-    pl->smem = pieces + pl->stages * per_stage;
     pl->grid = di.sms * per_sm;
     if (a->max_ctas > 0) pl->grid = std::min(pl->grid, a->max_ctas);
+    const int ring = kQ4Slots * 2 * 20 * a->head_dim;
+    pl->smem = pieces + kQ4Warps * ring;
+    // A warp's last piece is kept in its drained ring, and an item's merge keeps a weight for each
+    // head and CTA (and 16 bytes a thread) where the rings and pieces were.
+    const int merge = 4 * group * (pl->grid + 1) + 16 + 16 * kQ4Threads;
+    if (ring < q4_piece_bytes(group, a->head_dim) || merge > pl->smem || pl->smem > q4_max_smem(di, a->head_dim))
+        return fail(B2_ERR_UNSUPPORTED, "4-bit attention: shared memory");
     const size_t slots = 2 * static_cast<size_t>(pl->grid) * group;
     pl->ws_count = align_up(static_cast<size_t>(pl->grid) * sizeof(unsigned), 256);
     pl->ws_ml = align_up(slots * sizeof(float2), 256);
@@ -1697,7 +1698,7 @@ int launch_attn_q4_t(const Q4Plan& pl, const Q4AttnParams& p, cudaStream_t s) {
     static std::atomic<uint64_t> smem_set{0};
     int dev = -1;
     const DeviceInfo di = device_info(&dev);
-    const int rc = ensure_max_smem(kern, smem_set, dev, di.smem_per_sm / q4_ctas_per_sm(DH) - 1024 - 1536);
+    const int rc = ensure_max_smem(kern, smem_set, dev, q4_max_smem(di, DH));
     if (rc != B2_OK) return rc;
     return launch_pdl(kern, dim3(static_cast<unsigned>(pl.grid)), dim3(kQ4Threads), pl.smem, s, p);
 }
@@ -1799,12 +1800,10 @@ int b2_paged_attention_q4(const B2PagedAttnQ4Args* a, void* workspace, size_t wo
     p.window = a->window;
     p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
     p.softcap = a->softcap;
-    p.stages = pl.stages;
     unsigned up = 0;
     while ((1ull << up) < static_cast<unsigned long long>(a->n_kv_head)) ++up;
     p.kv_shift = 31 + up;
     p.kv_mul = static_cast<unsigned>(((1ull << (31 + up)) + a->n_kv_head - 1) / a->n_kv_head);
-    p.stages_log2 = pl.stages == 8 ? 3 : pl.stages == 4 ? 2 : 1;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.ws_count = reinterpret_cast<unsigned*>(ws);
     p.ws_ml = reinterpret_cast<float2*>(ws + pl.ws_count);
