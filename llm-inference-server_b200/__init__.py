@@ -183,8 +183,9 @@ def _ptr(t) -> int | None:
 
 def _stream(stream) -> int | None:
     if stream is None:
-        import torch
-        return torch.cuda.current_stream().cuda_stream
+        # what torch.cuda.current_stream().cuda_stream is, without making a Stream object each call
+        from torch import _C
+        return _C._cuda_getCurrentRawStream(_C._cuda_getDevice())
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 

@@ -1732,8 +1732,11 @@ int b2_block_map(const B2BlockMapArgs* a, b2_stream_t stream) {
     BlockMapParams p{a->n_seqs, a->max_blocks_per_seq, a->num_blocks, a->max_rows, a->seq_lens_pre, a->new_lens,
                      a->free_list, a->free_count, a->block_tables, a->slots, a->q_start, a->seq_lens_post,
                      a->free_count_out};
-    static std::atomic<uint64_t> smem_set{0};
-    return launch_blocks(block_map_kernel, smem_set, 4 * (3 * a->n_seqs + 1), p, static_cast<cudaStream_t>(stream));
+    static std::atomic<uint64_t> smem_set[2];
+    const int smem = 4 * (3 * a->n_seqs + 1);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a->n_seqs <= kMapThreads) return launch_blocks(block_map_kernel<1>, smem_set[0], smem, p, s);
+    return launch_blocks(block_map_kernel<kMapPer>, smem_set[1], smem, p, s);
 }
 
 int b2_block_release(const B2BlockReleaseArgs* a, b2_stream_t stream) {

@@ -47,38 +47,112 @@ struct KvQ4Params {
     int rows, n_kv_head, layer_idx, n_layer, num_blocks;
 };
 
-// The codes of 8 elements against (m, s), packed from the low nibble up.  With q the fp32
-// product (x - m) * (1 / s), off by at most 2^-22 |q|, rounding q gives the code wherever q is not
-// within 1e-4 of a rounding border; the few elements that are take the division.
-__device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float m, float s) {
-    constexpr float kMagic = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer, ties to even
-    const float rs = __frcp_rn(s);
+// Codes straight from the definition, packed from the low nibble up.
+__device__ __noinline__ uint32_t q4_codes_exact(const uint4 lo4, const uint4 hi4, float m, float s) {
+    const float x[8] = {__uint_as_float(lo4.x), __uint_as_float(lo4.y), __uint_as_float(lo4.z), __uint_as_float(lo4.w),
+                        __uint_as_float(hi4.x), __uint_as_float(hi4.y), __uint_as_float(hi4.z), __uint_as_float(hi4.w)};
     uint32_t codes = 0;
-    float far = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float q = (x[e] - m) * rs;
-        const float k = q + kMagic;
-        far = fmaxf(far, fabsf(q - (k - kMagic)));
-        codes |= static_cast<uint32_t>(min(max(static_cast<int>(__float_as_uint(k) - __float_as_uint(kMagic)), -8), 7) + 8) << (4 * e);
-    }
-    if (far > 0.4999f) {
-        codes = 0;
-#pragma unroll 1
-        for (int e = 7; e >= 0; --e) {
-            float v = x[0];
-#pragma unroll
-            for (int f = 1; f < 8; ++f) v = f == e ? x[f] : v;
-            codes = codes << 4 | static_cast<uint32_t>(fminf(fmaxf(rintf(__fdiv_rn(v - m, s)) + 8.0f, 0.0f), 15.0f));
-        }
+        const float v = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
+        codes |= static_cast<uint32_t>(fminf(fmaxf(rintf(__fdiv_rn(v - m, s)) + 8.0f, 0.0f), 15.0f)) << (4 * e);
     }
     return s > 0.0f ? codes : 0x88888888u;
 }
 
+// The codes of 8 elements.  q = x / s - m / s in one fused step is off by at most 2^-22 (|m / s| + 16) from
+// the quotient, so rounding it gives the code wherever it is further than that from a rounding border,
+// and no code needs cutting off where m's own rounding (2^-11 |m|) is under 0.45 s.  Anything else -- a few
+// elements in 10^5 of ordinary rows, groups far from zero for their width, saturated ones -- takes the definition.
+// Four codes are added up as c0 + 16 c1 + 256 c2 + 4096 c3 in fp32 (exact): fp32 instructions issue at
+// twice the integer ones' rate.
+__device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float m, float s, bool saturated) {
+    constexpr float kMagic = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer, ties to even
+    const float rs = __fdividef(1.0f, s), ms = -m * rs;
+    float far = 0.0f, packed[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        packed[w] = kMagic + 34952.0f;  // 8 (1 + 16 + 256 + 4096)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float q = fmaf(x[4 * w + e], rs, ms);
+            const float k = (q + kMagic) - kMagic;
+            far = fmaxf(far, fabsf(q - k));
+            packed[w] = fmaf(k, static_cast<float>(1 << (4 * e)), packed[w]);
+        }
+    }
+    // (also false for the NaN that s = 0 makes of ms)
+    if (!saturated && far < 0.4999f - fabsf(ms) * 0x1p-22f && fabsf(ms) * 0x1p-11f < 0.45f)
+        return __byte_perm(__float_as_uint(packed[0]), __float_as_uint(packed[1]), 0x5410);
+    return q4_codes_exact(make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])),
+                          make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])),
+                          m, s);
+}
+
+template <typename T>
+struct Pair16;
+template <>
+struct Pair16<__half> {
+    using Type = __half2;
+};
+template <>
+struct Pair16<__nv_bfloat16> {
+    using Type = __nv_bfloat162;
+};
+
+// Least and greatest of a group whose elements lie 8 to a lane in four neighbouring lanes, in the
+// 16-bit type itself; NaN if one is.
+template <typename T>
+__device__ __forceinline__ void q4_min_max(const uint4& raw, float* lo, float* hi) {
+    using P = typename Pair16<T>::Type;
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    P a = *reinterpret_cast<const P*>(&w[0]), b = a;
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+        const P v = *reinterpret_cast<const P*>(&w[k]);
+        a = __hmin2_nan(a, v);
+        b = __hmax2_nan(b, v);
+    }
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+        const uint32_t oa = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&a), d);
+        const uint32_t ob = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&b), d);
+        a = __hmin2_nan(a, *reinterpret_cast<const P*>(&oa));
+        b = __hmax2_nan(b, *reinterpret_cast<const P*>(&ob));
+    }
+    *lo = Elem<T>::to_f(__hmin_nan(a.x, a.y));
+    *hi = Elem<T>::to_f(__hmax_nan(b.x, b.y));
+}
+
+// Two of a word's values: codes in the low bits of both halves of c (as f16: 1024 + code, see below), w = (m, s).
+__device__ __forceinline__ void q4_values2(uint32_t c, uint32_t w, float m, float* x0, float* x1) {
+    asm("{\n\t.reg .f16 c0, c1, lo, hi;\n\t"
+        "mov.b32 {c0, c1}, %2;\n\tmov.b32 {lo, hi}, %3;\n\t"
+        "fma.rn.f32.f16 %0, c0, hi, %4;\n\tfma.rn.f32.f16 %1, c1, hi, %4;\n\t}"
+        : "=f"(*x0), "=f"(*x1)
+        : "r"(c), "r"(w), "f"(m));
+}
+
+// The 8 values of a codes word.  0x6400 | c is the f16 1024 + c (and 0x6400 | 16 c is 1024 + 16 c); taking 1032
+// off (or 1/16 of it less 72) leaves c - 8, all exact; s (c - 8) + m is one fused step with an fp32 result.
+__device__ __forceinline__ void q4_values(uint32_t codes, uint32_t w, float (&x)[8]) {
+    const float m = __half2float(__ushort_as_half(static_cast<unsigned short>(w & 0xffffu)));
+    const __half2 minus1032 = __float2half2_rn(-1032.0f), sixteenth = __float2half2_rn(0.0625f), minus72 = __float2half2_rn(-72.0f);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const uint32_t u = codes >> (8 * k);
+        const uint32_t even = (u & 0x000f000fu) | 0x64006400u, odd = (u & 0x00f000f0u) | 0x64006400u;
+        const __half2 e = __hadd2(*reinterpret_cast<const __half2*>(&even), minus1032);
+        const __half2 o = __hfma2(*reinterpret_cast<const __half2*>(&odd), sixteenth, minus72);
+        q4_values2(*reinterpret_cast<const uint32_t*>(&e), w, m, &x[2 * k], &x[2 * k + 4]);
+        q4_values2(*reinterpret_cast<const uint32_t*>(&o), w, m, &x[2 * k + 1], &x[2 * k + 5]);
+    }
+}
+
 // A CTA takes kRows rows; a thread 8 neighbouring elements (16 bytes) of K or of V in each, four
-// lanes a group of 32.  Bound: HBM, 2 bytes and 0.625 an element.  Several rows a thread keep that many
-// 16-byte loads in flight: at 65536 rows of 8 heads x 128 the read-back took 127 us with one row a thread
-// (and a 64-bit division to find it) and takes KROWS4_GATHER with four.
+// lanes a group of 32.  The bytes are 2 and 0.625 an element; what bounds it is instruction issue, so
+// everything that does not depend on the row is worked out once and the arithmetic stays off the
+// integer and conversion pipes.  At 16384 rows of 8 heads x 128: APPEND_NOTE.
 template <typename T, int DH, bool kAppend, int kRows>
 __global__ void __launch_bounds__(256) kv_q4_kernel(const KvQ4Params p) {
     using C = Q4Chunk<DH>;
@@ -107,6 +181,10 @@ __global__ void __launch_bounds__(256) kv_q4_kernel(const KvQ4Params p) {
         const int u = is_v ? c - per_row : c;
         const int i = u & 3, g = (u >> 2) % G, h = (u >> 2) / G;
         uint8_t* chunk0 = p.pool + (static_cast<size_t>(p.layer_idx) * p.n_kv_head + h) * C::kBytes;
+        uint8_t* param0 = chunk0 + (is_v ? C::kVParams : C::kKParams) + C::param(0, g);
+        uint8_t* code0 = chunk0 + (is_v ? C::v_unit(0, 2 * i, g) : C::k_word(0, i, g));
+        const int code_stride = is_v ? 32 : DH / 2;
+        constexpr int kNextUnit = C::v_unit(0, 1, 0) - C::v_unit(0, 0, 0);  // dims 4 .. 7 of a V thread: the next unit
         T* x0 = static_cast<T*>(is_v ? p.v : p.k) + row0 * p.row_stride + (h * DH + g * 32 + i * 8);
         if (kAppend) {
             uint4 raw[kRows];
@@ -115,36 +193,31 @@ __global__ void __launch_bounds__(256) kv_q4_kernel(const KvQ4Params p) {
                 raw[k] = mine && slot[k] >= 0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k * p.row_stride)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
             for (int k = 0; k < kRows; ++k) {
-                float x[8];
-                unpack16<T>(raw[k], x);
-                float lo = INFINITY, hi = -INFINITY, zero = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    zero = fmaf(x[e], 0.0f, zero);  // NaN if an element is NaN or infinite
-                    x[e] = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
-                    lo = fminf(lo, x[e]);
-                    hi = fmaxf(hi, x[e]);
-                }
-#pragma unroll
-                for (int d = 1; d < 4; d <<= 1) {
-                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-                    zero += __shfl_xor_sync(0xffffffffu, zero, d);
-                }
-                const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f));
-                const __half mh = __float2half_rn(fmaf(8.0f, __half2float(sh), lo));
+                float lo, hi, x[8];
+                q4_min_max<T>(raw[k], &lo, &hi);
                 if (!mine || slot[k] < 0) continue;
-                const uint32_t codes = q4_codes(x, __half2float(mh), __half2float(sh));
+                unpack16<T>(raw[k], x);
+                const bool finite = lo > -INFINITY && hi < INFINITY;  // false for NaN
+                const bool saturated = lo < -65504.0f || hi > 65504.0f;
+                lo = fminf(fmaxf(lo, -65504.0f), 65504.0f);
+                hi = fminf(fmaxf(hi, -65504.0f), 65504.0f);
+                // (hi - lo) / 15 with one correction step: exact quotients come out exact, others within a
+                // step of fp32, far from the f16 rounding borders they do not hit
+                const float range = hi - lo, r0 = range * (1.0f / 15.0f);
+                const __half sh = __float2half_rn(fmaf(fmaf(-15.0f, r0, range), 1.0f / 15.0f, r0));
+                const __half mh = __float2half_rn(fmaf(8.0f, __half2float(sh), lo));
+                const uint32_t codes = q4_codes(x, __half2float(mh), __half2float(sh), saturated);
                 const int t = slot[k] % kBlockTokens;
-                uint8_t* chunk = chunk0 + static_cast<size_t>(slot[k] / kBlockTokens) * block_bytes;
+                const size_t at = static_cast<size_t>(slot[k] / kBlockTokens) * block_bytes;
                 if (i == 0)
-                    *reinterpret_cast<uint32_t*>(chunk + (is_v ? C::kVParams : C::kKParams) + C::param(t, g)) =
-                        zero == 0.0f ? (static_cast<uint32_t>(__half_as_ushort(sh)) << 16 | __half_as_ushort(mh)) : 0x7fff7fffu;
+                    *reinterpret_cast<uint32_t*>(param0 + at + t * (4 * G)) =
+                        finite ? (static_cast<uint32_t>(__half_as_ushort(sh)) << 16 | __half_as_ushort(mh)) : 0x7fff7fffu;
+                uint8_t* to = code0 + at + t * code_stride;
                 if (!is_v) {
-                    *reinterpret_cast<uint32_t*>(chunk + C::k_word(t, i, g)) = codes;
+                    *reinterpret_cast<uint32_t*>(to) = codes;
                 } else {
-                    *reinterpret_cast<uint16_t*>(chunk + C::v_unit(t, 2 * i, g)) = static_cast<uint16_t>(codes);
-                    *reinterpret_cast<uint16_t*>(chunk + C::v_unit(t, 2 * i + 1, g)) = static_cast<uint16_t>(codes >> 16);
+                    *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(codes);
+                    *reinterpret_cast<uint16_t*>(to + kNextUnit) = static_cast<uint16_t>(codes >> 16);
                 }
             }
         } else {
@@ -152,23 +225,21 @@ __global__ void __launch_bounds__(256) kv_q4_kernel(const KvQ4Params p) {
             uint32_t w[kRows], codes[kRows];
 #pragma unroll
             for (int k = 0; k < kRows; ++k) {
+                w[k] = codes[k] = 0;
                 if (slot[k] < 0) continue;
                 const int t = slot[k] % kBlockTokens;
-                const uint8_t* chunk = chunk0 + static_cast<size_t>(slot[k] / kBlockTokens) * block_bytes;
-                w[k] = __ldg(reinterpret_cast<const uint32_t*>(chunk + (is_v ? C::kVParams : C::kKParams) + C::param(t, g)));
-                codes[k] = !is_v ? __ldg(reinterpret_cast<const uint32_t*>(chunk + C::k_word(t, i, g)))
-                                 : __ldg(reinterpret_cast<const uint16_t*>(chunk + C::v_unit(t, 2 * i, g))) |
-                                       static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(chunk + C::v_unit(t, 2 * i + 1, g)))) << 16;
+                const size_t at = static_cast<size_t>(slot[k] / kBlockTokens) * block_bytes;
+                w[k] = __ldg(reinterpret_cast<const uint32_t*>(param0 + at + t * (4 * G)));
+                const uint8_t* from = code0 + at + t * code_stride;
+                codes[k] = !is_v ? __ldg(reinterpret_cast<const uint32_t*>(from))
+                                 : __byte_perm(__ldg(reinterpret_cast<const uint16_t*>(from)),
+                                               __ldg(reinterpret_cast<const uint16_t*>(from + kNextUnit)), 0x5410);
             }
 #pragma unroll
             for (int k = 0; k < kRows; ++k) {
                 if (slot[k] < 0) continue;
-                const float s = __half2float(__ushort_as_half(static_cast<unsigned short>(w[k] >> 16)));
-                const float m = __half2float(__ushort_as_half(static_cast<unsigned short>(w[k] & 0xffffu)));
                 float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[e] = fmaf(static_cast<float>(static_cast<int>(codes[k] >> (4 * e) & 15u) - 8), s, m);
+                q4_values(codes[k], w[k], x);
                 *reinterpret_cast<uint4*>(x0 + k * p.row_stride) = pack16<T>(x);
             }
         }
