@@ -1593,20 +1593,37 @@ int check_q4_shape(int num_blocks, int n_layer, int n_kv_head, int head_dim) {
     return B2_OK;
 }
 
-// Four rows a CTA once that still gives every SM several CTAs; one below, where the call is
-// latency and more CTAs share it.  Threads: the fewest warps that take the same number of
-// rounds over a row pair's 16-byte pieces as 256 threads would.
-template <typename T, int DH, bool kAppend>
-int launch_kv_q4(const KvQ4Params& p, cudaStream_t s) {
-    int dev = -1;
-    const DeviceInfo di = device_info(&dev);
-    if (dev < 0 || di.sms <= 0) return fail(B2_ERR_DEVICE, "no current CUDA device");
+// Append: as many rows a CTA as give it up to 256 threads a pass (a thread takes a group of 32), fewer where
+// that leaves SMs without a CTA.
+template <typename T, int DH>
+int launch_append_q4(const KvQ4Params& p, const DeviceInfo& di, cudaStream_t s) {
+    const int per_row = 2 * p.n_kv_head * (DH / 32);
+    const int rows = std::max(1, std::min(256 / per_row, p.rows / di.sms));
+    const int threads = std::min(256, (rows * per_row + 31) / 32 * 32);
+    return launch_pdl(kv_append_q4_kernel<T, DH>, dim3(static_cast<unsigned>((p.rows + rows - 1ll) / rows)),
+                      dim3(static_cast<unsigned>(threads)), 0, s, p, rows);
+}
+
+// Read-back: four rows a CTA once that still gives every SM several CTAs; one below, where the call is
+// latency and more CTAs share it (1011 rows of 25 heads x 64: ROWS1 us with one, ROWS4 with four).  Threads:
+// the fewest warps that take the same number of rounds over a row pair's 16-byte pieces as 256 would.
+template <typename T, int DH>
+int launch_gather_q4(const KvQ4Params& p, const DeviceInfo& di, cudaStream_t s) {
     const int pieces = 2 * p.n_kv_head * (DH / 8);
     const int rounds = (pieces + 255) / 256;
     const dim3 threads(static_cast<unsigned>(((pieces + rounds - 1) / rounds + 31) / 32 * 32));
     if (p.rows >= 4 * 4 * di.sms)
-        return launch_pdl(kv_q4_kernel<T, DH, kAppend, 4>, dim3(static_cast<unsigned>((p.rows + 3ll) / 4)), threads, 0, s, p);
-    return launch_pdl(kv_q4_kernel<T, DH, kAppend, 1>, dim3(static_cast<unsigned>(p.rows)), threads, 0, s, p);
+        return launch_pdl(kv_gather_q4_kernel<T, DH, 4>, dim3(static_cast<unsigned>((p.rows + 3ll) / 4)), threads, 0, s, p);
+    return launch_pdl(kv_gather_q4_kernel<T, DH, 1>, dim3(static_cast<unsigned>(p.rows)), threads, 0, s, p);
+}
+
+template <bool kAppend, typename T>
+int launch_kv_q4(int head_dim, const KvQ4Params& p, cudaStream_t s) {
+    int dev = -1;
+    const DeviceInfo di = device_info(&dev);
+    if (dev < 0 || di.sms <= 0) return fail(B2_ERR_DEVICE, "no current CUDA device");
+    if (kAppend) return head_dim == 64 ? launch_append_q4<T, 64>(p, di, s) : launch_append_q4<T, 128>(p, di, s);
+    return head_dim == 64 ? launch_gather_q4<T, 64>(p, di, s) : launch_gather_q4<T, 128>(p, di, s);
 }
 
 template <bool kAppend>
@@ -1626,10 +1643,8 @@ int kv_q4(const B2KvQ4Args* a, b2_stream_t stream) {
     KvQ4Params p{static_cast<uint8_t*>(a->kv_pool), a->k, a->v, a->row_stride, a->slots, a->rows,
                  a->n_kv_head, a->layer_idx, a->n_layer, a->num_blocks};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a->dtype == B2_F16)
-        return a->head_dim == 64 ? launch_kv_q4<__half, 64, kAppend>(p, s) : launch_kv_q4<__half, 128, kAppend>(p, s);
-    return a->head_dim == 64 ? launch_kv_q4<__nv_bfloat16, 64, kAppend>(p, s)
-                             : launch_kv_q4<__nv_bfloat16, 128, kAppend>(p, s);
+    return a->dtype == B2_F16 ? launch_kv_q4<kAppend, __half>(a->head_dim, p, s)
+                              : launch_kv_q4<kAppend, __nv_bfloat16>(a->head_dim, p, s);
 }
 
 int check_attn_q4_args(const B2PagedAttnQ4Args* a) {

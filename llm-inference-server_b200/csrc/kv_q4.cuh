@@ -47,28 +47,27 @@ struct KvQ4Params {
     int rows, n_kv_head, layer_idx, n_layer, num_blocks;
 };
 
-// Codes straight from the definition, packed from the low nibble up.
-__device__ __noinline__ uint32_t q4_codes_exact(const uint4 lo4, const uint4 hi4, float m, float s) {
-    const float x[8] = {__uint_as_float(lo4.x), __uint_as_float(lo4.y), __uint_as_float(lo4.z), __uint_as_float(lo4.w),
-                        __uint_as_float(hi4.x), __uint_as_float(hi4.y), __uint_as_float(hi4.z), __uint_as_float(hi4.w)};
+// Codes of 8 elements straight from the definition, packed from the low nibble up; rs the correctly rounded 1 / s.
+// d rs with one correction step is the correctly rounded quotient (Markstein).
+__device__ __forceinline__ uint32_t q4_codes_exact(const float (&x)[8], float m, float s, float rs) {
     uint32_t codes = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float v = fminf(fmaxf(x[e], -65504.0f), 65504.0f);
-        codes |= static_cast<uint32_t>(fminf(fmaxf(rintf(__fdiv_rn(v - m, s)) + 8.0f, 0.0f), 15.0f)) << (4 * e);
+        const float d = fminf(fmaxf(x[e], -65504.0f), 65504.0f) - m;
+        const float q0 = d * rs, q = fmaf(fmaf(-q0, s, d), rs, q0);
+        codes |= static_cast<uint32_t>(static_cast<int>(rintf(fminf(fmaxf(q, -8.0f), 7.0f))) + 8) << (4 * e);
     }
-    return s > 0.0f ? codes : 0x88888888u;
+    return codes;
 }
 
-// The codes of 8 elements.  q = x / s - m / s in one fused step is off by at most 2^-22 (|m / s| + 16) from
-// the quotient, so rounding it gives the code wherever it is further than that from a rounding border,
-// and no code needs cutting off where m's own rounding (2^-11 |m|) is under 0.45 s.  Anything else -- a few
-// elements in 10^5 of ordinary rows, groups far from zero for their width, saturated ones -- takes the definition.
-// Four codes are added up as c0 + 16 c1 + 256 c2 + 4096 c3 in fp32 (exact): fp32 instructions issue at
-// twice the integer ones' rate.
-__device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float m, float s, bool saturated) {
+// The codes of 8 elements; rs = 1 / s, ms = -m / s.  q = x rs + ms in one fused step is off by at most 2^-22 (2 |ms| +
+// 16) from the quotient, so rounding it gives the code wherever it is further than that from a rounding
+// border, and no code needs cutting off where m's own rounding (2^-11 |m|) is under 0.45 s (`plain`).  Anything
+// else -- 0.06 % of the elements of normal bf16 rows, mostly exact ties; groups far from zero for their
+// width; saturated ones -- takes the definition.  Four codes are added up as c0 + 16 c1 + 256 c2 + 4096 c3 in
+// fp32 (exact): fp32 instructions issue at twice the integer ones' rate.
+__device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float m, float s, float rs, float ms, bool plain) {
     constexpr float kMagic = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer, ties to even
-    const float rs = __fdividef(1.0f, s), ms = -m * rs;
     float far = 0.0f, packed[2];
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
@@ -81,12 +80,9 @@ __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float m, float
             packed[w] = fmaf(k, static_cast<float>(1 << (4 * e)), packed[w]);
         }
     }
-    // (also false for the NaN that s = 0 makes of ms)
-    if (!saturated && far < 0.4999f - fabsf(ms) * 0x1p-22f && fabsf(ms) * 0x1p-11f < 0.45f)
+    if (plain && far < 0.49999f - fabsf(ms) * 0x1p-21f)
         return __byte_perm(__float_as_uint(packed[0]), __float_as_uint(packed[1]), 0x5410);
-    return q4_codes_exact(make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])),
-                          make_uint4(__float_as_uint(x[4]), __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7])),
-                          m, s);
+    return q4_codes_exact(x, m, s, rs);
 }
 
 template <typename T>
@@ -99,30 +95,6 @@ template <>
 struct Pair16<__nv_bfloat16> {
     using Type = __nv_bfloat162;
 };
-
-// Least and greatest of a group whose elements lie 8 to a lane in four neighbouring lanes, in the
-// 16-bit type itself; NaN if one is.
-template <typename T>
-__device__ __forceinline__ void q4_min_max(const uint4& raw, float* lo, float* hi) {
-    using P = typename Pair16<T>::Type;
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    P a = *reinterpret_cast<const P*>(&w[0]), b = a;
-#pragma unroll
-    for (int k = 1; k < 4; ++k) {
-        const P v = *reinterpret_cast<const P*>(&w[k]);
-        a = __hmin2_nan(a, v);
-        b = __hmax2_nan(b, v);
-    }
-#pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-        const uint32_t oa = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&a), d);
-        const uint32_t ob = __shfl_xor_sync(0xffffffffu, *reinterpret_cast<const uint32_t*>(&b), d);
-        a = __hmin2_nan(a, *reinterpret_cast<const P*>(&oa));
-        b = __hmax2_nan(b, *reinterpret_cast<const P*>(&ob));
-    }
-    *lo = Elem<T>::to_f(__hmin_nan(a.x, a.y));
-    *hi = Elem<T>::to_f(__hmax_nan(b.x, b.y));
-}
 
 // Two of a word's values: codes in the low bits of both halves of c (as f16: 1024 + code, see below), w = (m, s).
 __device__ __forceinline__ void q4_values2(uint32_t c, uint32_t w, float m, float* x0, float* x1) {
@@ -149,12 +121,84 @@ __device__ __forceinline__ void q4_values(uint32_t codes, uint32_t w, float (&x)
     }
 }
 
-// A CTA takes kRows rows; a thread 8 neighbouring elements (16 bytes) of K or of V in each, four
-// lanes a group of 32.  The bytes are 2 and 0.625 an element; what bounds it is instruction issue, so
-// everything that does not depend on the row is worked out once and the arithmetic stays off the
-// integer and conversion pipes.  At 16384 rows of 8 heads x 128: APPEND_NOTE.
-template <typename T, int DH, bool kAppend, int kRows>
-__global__ void __launch_bounds__(256) kv_q4_kernel(const KvQ4Params p) {
+// Quantising: a thread takes a whole group of 32 (64 bytes), so that what is per group -- extremes, step,
+// middle, their conversions -- is worked out once and no lanes have to agree.  2 bytes read and 0.625
+// written an element; what bounds it is instruction issue, about 11 an element (with four lanes to a
+// group: 25).  At 16384 rows of 8 heads x 128: APPEND_NOTE.
+template <typename T, int DH>
+__global__ void __launch_bounds__(256) kv_append_q4_kernel(const KvQ4Params p, int rows_per_cta) {
+    using C = Q4Chunk<DH>;
+    using P = typename Pair16<T>::Type;
+    constexpr int G = C::kGroups;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int per_row = 2 * p.n_kv_head * G;  // groups of a row's K and V
+    const size_t block_bytes = static_cast<size_t>(p.n_layer) * p.n_kv_head * C::kBytes;
+#pragma unroll 1
+    for (int idx = threadIdx.x; idx < rows_per_cta * per_row; idx += blockDim.x) {
+        const int local = idx / per_row, c = idx - local * per_row;
+        const long long row = static_cast<long long>(blockIdx.x) * rows_per_cta + local;
+        if (row >= p.rows) return;
+        const bool is_v = c >= per_row / 2;
+        const int u = is_v ? c - per_row / 2 : c;
+        const int g = u % G, h = u / G;
+        const int slot = __ldg(p.slots + row);
+        const T* from = static_cast<const T*>(is_v ? p.v : p.k) + row * p.row_stride + (h * DH + g * 32);
+        uint4 raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+        if (slot < 0) continue;
+        if (slot / kBlockTokens >= p.num_blocks) {
+            if (c == 0) flag_error(B2_DEVERR_BLOCK_ID);
+            continue;
+        }
+        // extremes in the 16-bit type itself; NaN if an element is
+        P a = *reinterpret_cast<const P*>(&raw[0].x), b = a;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                a = __hmin2_nan(a, *reinterpret_cast<const P*>(&w[k]));
+                b = __hmax2_nan(b, *reinterpret_cast<const P*>(&w[k]));
+            }
+        }
+        float lo = Elem<T>::to_f(__hmin_nan(a.x, a.y)), hi = Elem<T>::to_f(__hmax_nan(b.x, b.y));
+        const bool finite = lo > -INFINITY && hi < INFINITY;  // false for NaN
+        const bool saturated = lo < -65504.0f || hi > 65504.0f;
+        lo = fminf(fmaxf(lo, -65504.0f), 65504.0f);
+        hi = fminf(fmaxf(hi, -65504.0f), 65504.0f);
+        const __half sh = __float2half_rn(__fdiv_rn(hi - lo, 15.0f));
+        const float s = __half2float(sh);
+        const __half mh = __float2half_rn(fmaf(8.0f, s, lo));
+        const float m = __half2float(mh), rs = __frcp_rn(s), ms = -m * rs;
+        const bool plain = !saturated && fabsf(ms) * 0x1p-11f < 0.45f;  // also false for s = 0
+        const int t = slot % kBlockTokens;
+        uint8_t* chunk = p.pool + static_cast<size_t>(slot / kBlockTokens) * block_bytes +
+                         (static_cast<size_t>(p.layer_idx) * p.n_kv_head + h) * C::kBytes;
+        *reinterpret_cast<uint32_t*>(chunk + (is_v ? C::kVParams : C::kKParams) + C::param(t, g)) =
+            finite ? (static_cast<uint32_t>(__half_as_ushort(sh)) << 16 | __half_as_ushort(mh)) : 0x7fff7fffu;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x[8];
+            unpack16<T>(raw[i], x);
+            const uint32_t codes = s > 0.0f ? q4_codes(x, m, s, rs, ms, plain) : 0x88888888u;
+            if (!is_v) {
+                *reinterpret_cast<uint32_t*>(chunk + C::k_word(t, i, g)) = codes;
+            } else {
+                *reinterpret_cast<uint16_t*>(chunk + C::v_unit(t, 2 * i, g)) = static_cast<uint16_t>(codes);
+                *reinterpret_cast<uint16_t*>(chunk + C::v_unit(t, 2 * i + 1, g)) = static_cast<uint16_t>(codes >> 16);
+            }
+        }
+    }
+}
+
+// Reading back: a CTA takes kRows rows, a thread 8 neighbouring elements (16 bytes) of K or of V in each.  What
+// does not depend on the row is worked out once, and the arithmetic stays off the integer and conversion
+// pipes: 65531 rows of 8 heads x 128 took 127 us with one row a thread, 70 us with four, and take 66 us
+// (5.3 TB/s) without conversions.
+template <typename T, int DH, int kRows>
+__global__ void __launch_bounds__(256) kv_gather_q4_kernel(const KvQ4Params p) {
     using C = Q4Chunk<DH>;
     constexpr int G = C::kGroups;
     pdl_launch_dependents();
@@ -174,74 +218,35 @@ __global__ void __launch_bounds__(256) kv_q4_kernel(const KvQ4Params p) {
     if (err != 0 && threadIdx.x == 0) flag_error(err);
     const size_t block_bytes = static_cast<size_t>(p.n_layer) * p.n_kv_head * C::kBytes;
 #pragma unroll 1
-    for (int c0 = 0; c0 < 2 * per_row; c0 += blockDim.x) {  // whole warps: the shuffles need every lane
-        const int c = c0 + threadIdx.x;
-        const bool mine = c < 2 * per_row;
+    for (int c = threadIdx.x; c < 2 * per_row; c += blockDim.x) {
         const bool is_v = c >= per_row;
         const int u = is_v ? c - per_row : c;
         const int i = u & 3, g = (u >> 2) % G, h = (u >> 2) / G;
-        uint8_t* chunk0 = p.pool + (static_cast<size_t>(p.layer_idx) * p.n_kv_head + h) * C::kBytes;
-        uint8_t* param0 = chunk0 + (is_v ? C::kVParams : C::kKParams) + C::param(0, g);
-        uint8_t* code0 = chunk0 + (is_v ? C::v_unit(0, 2 * i, g) : C::k_word(0, i, g));
+        const uint8_t* chunk0 = p.pool + (static_cast<size_t>(p.layer_idx) * p.n_kv_head + h) * C::kBytes;
+        const uint8_t* param0 = chunk0 + (is_v ? C::kVParams : C::kKParams) + C::param(0, g);
+        const uint8_t* code0 = chunk0 + (is_v ? C::v_unit(0, 2 * i, g) : C::k_word(0, i, g));
         const int code_stride = is_v ? 32 : DH / 2;
         constexpr int kNextUnit = C::v_unit(0, 1, 0) - C::v_unit(0, 0, 0);  // dims 4 .. 7 of a V thread: the next unit
         T* x0 = static_cast<T*>(is_v ? p.v : p.k) + row0 * p.row_stride + (h * DH + g * 32 + i * 8);
-        if (kAppend) {
-            uint4 raw[kRows];
+        uint32_t w[kRows], codes[kRows];
 #pragma unroll
-            for (int k = 0; k < kRows; ++k)
-                raw[k] = mine && slot[k] >= 0 ? __ldg(reinterpret_cast<const uint4*>(x0 + k * p.row_stride)) : make_uint4(0, 0, 0, 0);
+        for (int k = 0; k < kRows; ++k) {
+            w[k] = codes[k] = 0;
+            if (slot[k] < 0) continue;
+            const int t = slot[k] % kBlockTokens;
+            const size_t at = static_cast<size_t>(slot[k] / kBlockTokens) * block_bytes;
+            w[k] = __ldg(reinterpret_cast<const uint32_t*>(param0 + at + t * (4 * G)));
+            const uint8_t* from = code0 + at + t * code_stride;
+            codes[k] = !is_v ? __ldg(reinterpret_cast<const uint32_t*>(from))
+                             : __byte_perm(__ldg(reinterpret_cast<const uint16_t*>(from)),
+                                           __ldg(reinterpret_cast<const uint16_t*>(from + kNextUnit)), 0x5410);
+        }
 #pragma unroll
-            for (int k = 0; k < kRows; ++k) {
-                float lo, hi, x[8];
-                q4_min_max<T>(raw[k], &lo, &hi);
-                if (!mine || slot[k] < 0) continue;
-                unpack16<T>(raw[k], x);
-                const bool finite = lo > -INFINITY && hi < INFINITY;  // false for NaN
-                const bool saturated = lo < -65504.0f || hi > 65504.0f;
-                lo = fminf(fmaxf(lo, -65504.0f), 65504.0f);
-                hi = fminf(fmaxf(hi, -65504.0f), 65504.0f);
-                // (hi - lo) / 15 with one correction step: exact quotients come out exact, others within a
-                // step of fp32, far from the f16 rounding borders they do not hit
-                const float range = hi - lo, r0 = range * (1.0f / 15.0f);
-                const __half sh = __float2half_rn(fmaf(fmaf(-15.0f, r0, range), 1.0f / 15.0f, r0));
-                const __half mh = __float2half_rn(fmaf(8.0f, __half2float(sh), lo));
-                const uint32_t codes = q4_codes(x, __half2float(mh), __half2float(sh), saturated);
-                const int t = slot[k] % kBlockTokens;
-                const size_t at = static_cast<size_t>(slot[k] / kBlockTokens) * block_bytes;
-                if (i == 0)
-                    *reinterpret_cast<uint32_t*>(param0 + at + t * (4 * G)) =
-                        finite ? (static_cast<uint32_t>(__half_as_ushort(sh)) << 16 | __half_as_ushort(mh)) : 0x7fff7fffu;
-                uint8_t* to = code0 + at + t * code_stride;
-                if (!is_v) {
-                    *reinterpret_cast<uint32_t*>(to) = codes;
-                } else {
-                    *reinterpret_cast<uint16_t*>(to) = static_cast<uint16_t>(codes);
-                    *reinterpret_cast<uint16_t*>(to + kNextUnit) = static_cast<uint16_t>(codes >> 16);
-                }
-            }
-        } else {
-            if (!mine) continue;
-            uint32_t w[kRows], codes[kRows];
-#pragma unroll
-            for (int k = 0; k < kRows; ++k) {
-                w[k] = codes[k] = 0;
-                if (slot[k] < 0) continue;
-                const int t = slot[k] % kBlockTokens;
-                const size_t at = static_cast<size_t>(slot[k] / kBlockTokens) * block_bytes;
-                w[k] = __ldg(reinterpret_cast<const uint32_t*>(param0 + at + t * (4 * G)));
-                const uint8_t* from = code0 + at + t * code_stride;
-                codes[k] = !is_v ? __ldg(reinterpret_cast<const uint32_t*>(from))
-                                 : __byte_perm(__ldg(reinterpret_cast<const uint16_t*>(from)),
-                                               __ldg(reinterpret_cast<const uint16_t*>(from + kNextUnit)), 0x5410);
-            }
-#pragma unroll
-            for (int k = 0; k < kRows; ++k) {
-                if (slot[k] < 0) continue;
-                float x[8];
-                q4_values(codes[k], w[k], x);
-                *reinterpret_cast<uint4*>(x0 + k * p.row_stride) = pack16<T>(x);
-            }
+        for (int k = 0; k < kRows; ++k) {
+            if (slot[k] < 0) continue;
+            float x[8];
+            q4_values(codes[k], w[k], x);
+            *reinterpret_cast<uint4*>(x0 + k * p.row_stride) = pack16<T>(x);
         }
     }
 }
