@@ -1573,14 +1573,14 @@ namespace {
 
 // Cluster kernels of blocks.cuh: shared bytes above the default need the opt-in.
 template <typename K, typename P>
-int launch_blocks(K kern, std::atomic<uint64_t>& smem_set, int smem, const P& prm, cudaStream_t stream) {
+int launch_blocks(K kern, std::atomic<uint64_t>& smem_set, int smem, const P& prm, cudaStream_t stream, int clusters = 1) {
     int dev = -1;
     const DeviceInfo di = device_info(&dev);
     if (dev < 0) return fail(B2_ERR_DEVICE, "no current CUDA device");
     // The limit, less the kernels' static shared memory.
     const int rc = ensure_max_smem(kern, smem_set, dev, di.max_smem_optin - 1024);
     if (rc != B2_OK) return rc;
-    return launch_pdl(kern, dim3(kMapCluster), dim3(kMapThreads), smem, stream, prm);
+    return launch_pdl(kern, dim3(static_cast<unsigned>(clusters * kMapCluster)), dim3(kMapThreads), smem, stream, prm);
 }
 
 // The largest slot is below 2^31, and the chunk index (block, layer, head) too.
@@ -1750,8 +1750,12 @@ int b2_block_map(const B2BlockMapArgs* a, b2_stream_t stream) {
     static std::atomic<uint64_t> smem_set[2];
     const int smem = 4 * (3 * a->n_seqs + 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (a->n_seqs <= kMapThreads) return launch_blocks(block_map_kernel<1>, smem_set[0], smem, p, s);
-    return launch_blocks(block_map_kernel<kMapPer>, smem_set[1], smem, p, s);
+    // One cluster maps four rows a thread in one pass; updates in place need a single one.
+    const bool in_place = a->seq_lens_post == a->seq_lens_pre || a->free_count_out == a->free_count;
+    const int passes = (a->max_rows + 4 * kMapCluster * kMapThreads - 1) / (4 * kMapCluster * kMapThreads);
+    const int clusters = in_place ? 1 : std::max(1, std::min(8, passes));
+    if (a->n_seqs <= kMapThreads) return launch_blocks(block_map_kernel<1>, smem_set[0], smem, p, s, clusters);
+    return launch_blocks(block_map_kernel<kMapPer>, smem_set[1], smem, p, s, clusters);
 }
 
 int b2_block_release(const B2BlockReleaseArgs* a, b2_stream_t stream) {

@@ -4,11 +4,13 @@
 // Two prefix sums over the sequences carry both operators: rows (or blocks to
 // give back) before sequence b, and blocks needed before sequence b.  What
 // bounds them is latency -- a launch, a chain of dependent loads, two scans -- not
-// the few hundred KB they move, so each is one launch of one thread-block
-// cluster: every CTA reads all lengths and scans them for itself (n <= 16384
-// values, a few L2 lines a thread) and then writes its share of the rows.  Only
-// free_count and the lengths may be updated in place; every CTA has read them
-// before the cluster barrier, and they are written after it.
+// the few hundred KB they move, so each is one launch, of thread-block clusters:
+// every CTA reads all lengths and scans them for itself (n <= 16384 values, a
+// few L2 lines a thread) and then writes its share of the rows.  Only
+// free_count and the lengths may be updated in place; then there is one cluster,
+// every CTA of which has read them before its barrier, and they are written
+// after it.  Into separate outputs the map of many rows takes more clusters (512
+// prompts, 139 k rows: MAP1 us with one, MAPN with eight).
 #pragma once
 
 #include <cooperative_groups.h>
@@ -21,6 +23,7 @@ constexpr int kMapThreads = 1024;
 constexpr int kMapCluster = 8;  // the portable cluster size
 constexpr int kMapMaxSeqs = B2_MAP_MAX_SEQS;
 constexpr int kMapPer = kMapMaxSeqs / kMapThreads;  // sequences per thread at most
+constexpr int kMapKept = 8;
 constexpr unsigned kMapRefused = 0x80000000u;
 // Sums are cut off here (far above any free_count): a + b of two cut sums fits
 // 32 bits, and min(a + b, cap) is associative.
@@ -122,7 +125,7 @@ block_map_kernel(const BlockMapParams p) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x;
-    const int rank = static_cast<int>(cluster.block_rank());
+    const int rank = static_cast<int>(blockIdx.x);
     pdl_launch_dependents();
     pdl_wait();
     if (tid == 0) s_used = 0;
@@ -192,12 +195,14 @@ block_map_kernel(const BlockMapParams p) {
         }
     }
     if (used != 0) atomicMax(&s_used, used);  // the same value whatever the order
-    cluster.sync();  // also the CTA's barrier: s_* are complete; every CTA has read lengths and count
+    // Also the CTA's barrier: s_* are complete.  Where lengths or count are updated in place there is one
+    // cluster, and every CTA has read them now.
+    cluster.sync();
 
     // rows, four to a thread: one binary search, one 16-byte store
     const int quads = (p.max_rows + 3) / 4;
     const int total = static_cast<int>(total_rows);
-    for (int q = rank * kMapThreads + tid; q < quads; q += kMapCluster * kMapThreads) {
+    for (int q = rank * kMapThreads + tid; q < quads; q += static_cast<int>(gridDim.x) * kMapThreads) {
         int out[4];
         int b = -1, blk_at = -1, id = -1;
 #pragma unroll
@@ -304,7 +309,8 @@ block_release_kernel(const BlockReleaseParams p) {
         }
     if (tid == 0) s_first[n] = total;
     __syncthreads();
-    for (unsigned e = tid; e < total; e += kMapThreads) {
+    // The first kMapKept ids of a thread stay in registers until their places are known.
+    auto id_of = [&](unsigned e) {
         const int i = last_at_most(s_first, n, e);
         const int id = __ldg(p.tables + static_cast<size_t>(lo + i) * p.mbps + (e - s_first[i]));
         if (id < 0 || id >= p.num_blocks) {
@@ -312,7 +318,16 @@ block_release_kernel(const BlockReleaseParams p) {
             s_any_bad = 1;
             err |= B2_DEVERR_BLOCK_ID;
         }
+        return id;
+    };
+    int kept[kMapKept];
+#pragma unroll
+    for (int k = 0; k < kMapKept; ++k) {
+        const unsigned e = tid + k * kMapThreads;
+        kept[k] = e < total ? id_of(e) : -1;
     }
+#pragma unroll 1
+    for (unsigned e = tid + kMapKept * kMapThreads; e < total; e += kMapThreads) id_of(e);
     __syncthreads();
     const bool any_bad = s_any_bad != 0;
     unsigned good = total;
@@ -335,11 +350,14 @@ block_release_kernel(const BlockReleaseParams p) {
     const unsigned room = static_cast<unsigned>(p.num_blocks);
     if (end > room) err |= B2_DEVERR_BLOCK_ID;
     if (!any_bad) {
-        for (unsigned e = tid; e < total; e += kMapThreads) {
-            const int i = last_at_most(s_first, n, e);
-            const int id = __ldg(p.tables + static_cast<size_t>(lo + i) * p.mbps + (e - s_first[i]));
-            if (base + e < room) p.free_list[base + e] = id;
+#pragma unroll
+        for (int k = 0; k < kMapKept; ++k) {
+            const unsigned e = tid + k * kMapThreads;
+            if (e < total && base + e < room) p.free_list[base + e] = kept[k];
         }
+#pragma unroll 1
+        for (unsigned e = tid + kMapKept * kMapThreads; e < total; e += kMapThreads)
+            if (base + e < room) p.free_list[base + e] = id_of(e);
     } else {  // rare: a thread closes the gaps of its own sequences
         unsigned at = base + first;
 #pragma unroll
