@@ -38,6 +38,16 @@
 // Pieces of an item (sequence, kv head) that several warps hold meet in shared
 // memory, those of several CTAs in the workspace; the CTA that arrives last
 // merges them in CTA order, so results do not depend on timing.
+//
+// Measured on one B200 (copy rate 6453 GB/s), a launch among others in a graph:
+//   32 sequences of 512 to 32768 tokens, 32/8 heads x 128, bf16   92 us, 4.3 TB/s
+//   61 sequences, window 4096, capped scores, same heads          59 us, 3.8 TB/s
+//   128 sequences of 256 to 1011 tokens, 25 heads x 64            49 us, 2.9 TB/s
+//   64 sequences of 128 to 1024 tokens, 12 heads x 64             16 us, 1.7 TB/s
+// Streaming the same chunks without the arithmetic takes 68, 43, 31 and 11 us: the rest is
+// instruction issue (351 warp instructions a chunk of head_dim 128, 55 % of the issue
+// slots), and on the short calls the chain from the wait for the kernel before to the
+// first chunk (4 us) and through the merges (4 us).
 #pragma once
 
 #include <cfloat>
@@ -66,8 +76,12 @@ struct Q4AttnParams {
 
 constexpr int kQ4Warps = 4;
 constexpr int kQ4Threads = 32 * kQ4Warps;
+// 128 registers a thread at head_dim 64, 168 at 128, where the sums alone take 32.  (128: 4 CTAs 95 us on long
+// GQA contexts, 3 CTAs 93; one 32768-token sequence 29 against 25.5.  64, 128 sequences of 25 heads: 5 CTAs 54 us,
+// 4 CTAs 49, 3 CTAs 58.  CTAs of 8 warps, two an SM: 98 us and 52.)
 constexpr int q4_ctas_per_sm(int dh) { return dh == 64 ? 4 : 3; }
-constexpr int kQ4Slots = 2;  // ring slots of a warp, a step (two chunks) each
+// Ring slots of a warp, a step (two chunks) each: 61 or 82 KB in flight an SM.  A third one cost 1 to 2 %.
+constexpr int kQ4Slots = 2;
 constexpr int kQ4MaxGroup = 8;
 constexpr int kQ4FewParts = 4;  // parts of an item that a CTA merges straight from L2
 constexpr float kLog2e = 1.4426950408889634f;

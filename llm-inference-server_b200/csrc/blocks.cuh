@@ -10,7 +10,7 @@
 // free_count and the lengths may be updated in place; then there is one cluster,
 // every CTA of which has read them before its barrier, and they are written
 // after it.  Into separate outputs the map of many rows takes more clusters (512
-// prompts, 139 k rows: MAP1 us with one, MAPN with eight).
+// prompts, 139 k rows: 13.7 us with one, 7.4 with five).
 #pragma once
 
 #include <cooperative_groups.h>
@@ -112,7 +112,7 @@ __device__ __forceinline__ int read_free_count(const int* p, int num_blocks, uns
 
 // Shared words: row[n + 1], blk[n], pre[n].  kPer: sequences to a thread, at most; small calls take the
 // kernel for one (the loops over them are unrolled, and a launch that is all latency pays for
-// every instruction it fetches: 64 sequences 6.4 -> MAP64 us).
+// every instruction it fetches: 64 sequences 6.4 -> 4.8 us).
 template <int kPer>
 __global__ void __cluster_dims__(kMapCluster, 1, 1) __launch_bounds__(kMapThreads)
 block_map_kernel(const BlockMapParams p) {
