@@ -610,6 +610,7 @@ B2_API int b2_kv_gather_q4(const B2KvQ4Args* args, b2_stream_t stream);
  * key_starts masks the keys in front of the query's own document (or a
  * left-padded batch's padding).  A sequence without visible keys gets zeros.
  * q and out F16 or BF16 (out also F32); any n_head / n_kv_head from 1 to 8.
+ * |q| up to 2^110: beyond, scores overflow to NaN.
  * A seq_len beyond max_blocks_per_seq * 16 or below 0 is clamped
  * (B2_DEVERR_SEQ_LEN), a block id outside the pool is clamped
  * (B2_DEVERR_BLOCK_ID).
