@@ -529,8 +529,8 @@ B2_API int b2_block_map(const B2BlockMapArgs* args, b2_stream_t stream);
  * for tables that live on the device.  Table entries are not cleared.  A
  * block must belong to one sequence only.  An id outside [0, num_blocks) sets
  * B2_DEVERR_BLOCK_ID and is left out; ids that would go past num_blocks entries
- * (something was given back twice) set it too and are dropped.  A seq_len
- * outside [0, max_blocks_per_seq * 16] is clamped into it and sets
+ * (something was given back twice) set it too and are dropped.  A released
+ * seq_len outside [0, max_blocks_per_seq * 16] is clamped into it and sets
  * B2_DEVERR_SEQ_LEN.  seq_lens_out may be seq_lens, free_count_out may be
  * free_count; no other two arrays may overlap.  n_seqs <= B2_MAP_MAX_SEQS.
  * One launch of one thread-block cluster. */
@@ -618,8 +618,9 @@ B2_API int b2_kv_gather_q4(const B2KvQ4Args* args, b2_stream_t stream);
  * The work is split evenly over the GPU by blocks; partial results meet in
  * the workspace.  Size it with b2_paged_attention_q4_workspace_bytes and zero it
  * once; every launch leaves its counters at zero (zero it again after
- * B2_DEVERR_TIMEOUT).  Launches that may overlap need a workspace each --
- * captured graphs that may run at the same time included. */
+ * B2_DEVERR_TIMEOUT).  Launches of different shapes may share one that is large
+ * enough for each.  Launches that may overlap need a workspace each -- captured
+ * graphs that may run at the same time included. */
 typedef struct B2PagedAttnQ4Args {
     int32_t dtype;     /* B2_F16 or B2_BF16: q */
     int32_t out_dtype; /* B2_F32, or the same as dtype */

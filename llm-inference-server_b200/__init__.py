@@ -181,11 +181,17 @@ def _ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_current = None
+
+
 def _stream(stream) -> int | None:
     if stream is None:
         # what torch.cuda.current_stream().cuda_stream is, without making a Stream object each call
-        from torch import _C
-        return _C._cuda_getCurrentRawStream(_C._cuda_getDevice())
+        global _current
+        if _current is None:
+            from torch import _C
+            _current = (_C._cuda_getCurrentRawStream, _C._cuda_getDevice)
+        return _current[0](_current[1]())
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 

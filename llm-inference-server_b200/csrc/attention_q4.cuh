@@ -66,7 +66,7 @@ struct Q4AttnParams {
     const int* key_starts;
     const float* slopes;
     void* out;
-    unsigned* ws_count;  // [grid]
+    unsigned* ws_count;  // [kQ4MaxCtas]
     float2* ws_ml;       // [2 grid][group]
     float* ws_acc;       // [2 grid][group][head_dim]
     int batch, n_head, n_kv_head, group, mbps, layer_idx, n_layer, num_blocks, window;
@@ -82,6 +82,7 @@ constexpr int kQ4Threads = 32 * kQ4Warps;
 constexpr int q4_ctas_per_sm(int dh) { return dh == 64 ? 4 : 3; }
 // Ring slots of a warp, a step (two chunks) each: 61 or 82 KB in flight an SM.  A third one cost 1 to 2 %.
 constexpr int kQ4Slots = 2;
+constexpr int kQ4MaxCtas = 1024;  // the workspace's counters: as many whatever the call's shape, so that calls of different shapes may share one
 constexpr int kQ4MaxGroup = 8;
 constexpr int kQ4FewParts = 4;  // parts of an item that a CTA merges straight from L2
 constexpr float kLog2e = 1.4426950408889634f;
@@ -91,13 +92,13 @@ __host__ __device__ constexpr int q4_piece_bytes(int group, int dh) { return (gr
 
 // Visible keys of a sequence: [first, n).
 __device__ __forceinline__ void q4_range(const Q4AttnParams& p, int b, int* first, int* n, unsigned* err) {
-    int len = __ldg(p.seq_lens + b);
+    int len = *(p.seq_lens + b);
     if (len < 0 || len > p.mbps * kBlockTokens) {
         *err |= B2_DEVERR_SEQ_LEN;
         len = min(max(len, 0), p.mbps * kBlockTokens);
     }
     int lo = 0;
-    if (p.key_starts != nullptr) lo = max(lo, __ldg(p.key_starts + b));
+    if (p.key_starts != nullptr) lo = max(lo, *(p.key_starts + b));
     if (p.window > 0) lo = max(lo, len - p.window);
     *first = min(lo, len);
     *n = len;
@@ -186,7 +187,7 @@ __device__ __forceinline__ void q4_start(const Q4AttnParams& p, int b, int hk, Q
     for (int g = 0; g < G; ++g) {
         uint4 raw = make_uint4(0, 0, 0, 0);
         if (r < p.group)
-            raw = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_row_stride +
+            raw = *(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_row_stride +
                                                        static_cast<long long>(hk * p.group + r) * DH + g * 32 + i * 8));
         unpack16<T>(raw, x[g]);
 #pragma unroll
@@ -225,7 +226,7 @@ __device__ __forceinline__ void q4_start(const Q4AttnParams& p, int b, int hk, Q
     for (int h = 0; h < 2; ++h) {
         const int src = 4 * (2 * i + h);
         st.sc[h] = __shfl_sync(0xffffffffu, sc, src);
-        st.slope[h] = p.slopes != nullptr && 2 * i + h < p.group ? __ldg(p.slopes + hk * p.group + 2 * i + h) * kLog2e : 0.0f;
+        st.slope[h] = p.slopes != nullptr && 2 * i + h < p.group ? *(p.slopes + hk * p.group + 2 * i + h) * kLog2e : 0.0f;
         st.ref[h] = -FLT_MAX;
         st.l[h] = 0.0f;
     }
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q
             const int blk = first / kBlockTokens + 2 * (static_cast<int>(c - base) - h * steps);
             const int* entry = p.block_tables + static_cast<size_t>(b) * p.mbps + blk;
             const bool two = (blk + 1) * kBlockTokens < n;
-            int id[2] = {__ldg(entry), two ? __ldg(entry + 1) : 0};
+            int id[2] = {*entry, two ? *(entry + 1) : 0};
             int4 step = make_int4(0, -1, b * p.n_kv_head + h, blk);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {

@@ -1691,7 +1691,7 @@ int plan_attn_q4(const B2PagedAttnQ4Args* a, Q4Plan* pl) {
     if (dev < 0 || di.sms <= 0) return fail(B2_ERR_DEVICE, "no current CUDA device");
     const int group = a->n_head / a->n_kv_head, per_sm = q4_ctas_per_sm(a->head_dim);
     const int pieces = kQ4Warps * q4_piece_bytes(group, a->head_dim);
-    pl->grid = di.sms * per_sm;
+    pl->grid = std::min(di.sms * per_sm, kQ4MaxCtas);
     if (a->max_ctas > 0) pl->grid = std::min(pl->grid, a->max_ctas);
     const int ring = kQ4Slots * 2 * 20 * a->head_dim;
     pl->smem = pieces + kQ4Warps * ring;
@@ -1701,7 +1701,7 @@ int plan_attn_q4(const B2PagedAttnQ4Args* a, Q4Plan* pl) {
     if (ring < q4_piece_bytes(group, a->head_dim) || merge > pl->smem || pl->smem > q4_max_smem(di, a->head_dim))
         return fail(B2_ERR_UNSUPPORTED, "4-bit attention: shared memory");
     const size_t slots = 2 * static_cast<size_t>(pl->grid) * group;
-    pl->ws_count = align_up(static_cast<size_t>(pl->grid) * sizeof(unsigned), 256);
+    pl->ws_count = kQ4MaxCtas * sizeof(unsigned);
     pl->ws_ml = align_up(slots * sizeof(float2), 256);
     pl->ws_total = pl->ws_count + pl->ws_ml + align_up(slots * a->head_dim * sizeof(float), 256);
     return B2_OK;

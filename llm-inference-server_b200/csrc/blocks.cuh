@@ -143,7 +143,7 @@ block_map_kernel(const BlockMapParams p) {
     for (int i = 0; i < kPer; ++i) {
         add[i] = 0;
         if (b0 + i < b1) {
-            const int a = p.added != nullptr ? __ldg(p.added + b0 + i) : 1;
+            const int a = p.added != nullptr ? *(p.added + b0 + i) : 1;
             s_pre[b0 + i] = p.pre[b0 + i];
             add[i] = a;
             rows = sat_add(rows, min(static_cast<unsigned>(max(a, 0)), row_cap), row_cap);
@@ -223,7 +223,7 @@ block_map_kernel(const BlockMapParams p) {
             int* entry = p.tables + static_cast<size_t>(b) * p.mbps + at;
             if (at != blk_at) {
                 blk_at = at;
-                id = at < have ? *entry : __ldg(p.free_list + (free_count - 1 - static_cast<int>(base) - (at - have)));
+                id = at < have ? *entry : *(p.free_list + (free_count - 1 - static_cast<int>(base) - (at - have)));
                 if (id < 0 || id >= p.num_blocks) err |= B2_DEVERR_BLOCK_ID;
             }
             // the first position of a new block is always one of the new rows
@@ -289,7 +289,7 @@ block_release_kernel(const BlockReleaseParams p) {
             const int b = lo + i0 + k;
             const int len = p.lens[b];
             const int cut = min(max(len, 0), p.mbps * kBlockTokens);
-            if (__ldg(p.release + b) != 0) {
+            if (*(p.release + b) != 0) {
                 have[k] = static_cast<unsigned>(blocks_of(cut));
                 if (cut != len) err |= B2_DEVERR_SEQ_LEN;
             } else {
@@ -312,7 +312,7 @@ block_release_kernel(const BlockReleaseParams p) {
     // The first kMapKept ids of a thread stay in registers until their places are known.
     auto id_of = [&](unsigned e) {
         const int i = last_at_most(s_first, n, e);
-        const int id = __ldg(p.tables + static_cast<size_t>(lo + i) * p.mbps + (e - s_first[i]));
+        const int id = *(p.tables + static_cast<size_t>(lo + i) * p.mbps + (e - s_first[i]));
         if (id < 0 || id >= p.num_blocks) {
             atomicAdd(&s_bad[i], 1u);
             s_any_bad = 1;
@@ -363,7 +363,7 @@ block_release_kernel(const BlockReleaseParams p) {
 #pragma unroll
         for (int k = 0; k < kPer; ++k)
             for (unsigned c = 0; c < have[k]; ++c) {
-                const int id = __ldg(p.tables + static_cast<size_t>(lo + i0 + k) * p.mbps + c);
+                const int id = *(p.tables + static_cast<size_t>(lo + i0 + k) * p.mbps + c);
                 if (id < 0 || id >= p.num_blocks) continue;
                 if (at < room) p.free_list[at] = id;
                 ++at;

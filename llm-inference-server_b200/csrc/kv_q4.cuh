@@ -142,11 +142,11 @@ __global__ void __launch_bounds__(256) kv_append_q4_kernel(const KvQ4Params p, i
         const bool is_v = c >= per_row / 2;
         const int u = is_v ? c - per_row / 2 : c;
         const int g = u % G, h = u / G;
-        const int slot = __ldg(p.slots + row);
+        const int slot = *(p.slots + row);
         const T* from = static_cast<const T*>(is_v ? p.v : p.k) + row * p.row_stride + (h * DH + g * 32);
         uint4 raw[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+        for (int i = 0; i < 4; ++i) raw[i] = *(reinterpret_cast<const uint4*>(from) + i);
         if (slot < 0) continue;
         if (slot / kBlockTokens >= p.num_blocks) {
             if (c == 0) flag_error(B2_DEVERR_BLOCK_ID);
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(256) kv_gather_q4_kernel(const KvQ4Params p) {
     unsigned err = 0;
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-        slot[k] = row0 + k < p.rows ? __ldg(p.slots + row0 + k) : -1;
+        slot[k] = row0 + k < p.rows ? *(p.slots + row0 + k) : -1;
         if (slot[k] >= 0 && slot[k] / kBlockTokens >= p.num_blocks) {
             err |= B2_DEVERR_BLOCK_ID;
             slot[k] = -1;
@@ -235,11 +235,11 @@ __global__ void __launch_bounds__(256) kv_gather_q4_kernel(const KvQ4Params p) {
             if (slot[k] < 0) continue;
             const int t = slot[k] % kBlockTokens;
             const size_t at = static_cast<size_t>(slot[k] / kBlockTokens) * block_bytes;
-            w[k] = __ldg(reinterpret_cast<const uint32_t*>(param0 + at + t * (4 * G)));
+            w[k] = *(reinterpret_cast<const uint32_t*>(param0 + at + t * (4 * G)));
             const uint8_t* from = code0 + at + t * code_stride;
-            codes[k] = !is_v ? __ldg(reinterpret_cast<const uint32_t*>(from))
-                             : __byte_perm(__ldg(reinterpret_cast<const uint16_t*>(from)),
-                                           __ldg(reinterpret_cast<const uint16_t*>(from + kNextUnit)), 0x5410);
+            codes[k] = !is_v ? *reinterpret_cast<const uint32_t*>(from)
+                             : __byte_perm(*reinterpret_cast<const uint16_t*>(from),
+                                           *reinterpret_cast<const uint16_t*>(from + kNextUnit), 0x5410);
         }
 #pragma unroll
         for (int k = 0; k < kRows; ++k) {

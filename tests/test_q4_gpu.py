@@ -541,6 +541,45 @@ def test_workspace_is_checked(b2, cuda):
     assert e.value.code == -5
 
 
+def test_calls_of_different_shapes_share_a_workspace(b2, cuda):
+    torch = _torch()
+    names = ["gqa4", "microbench", "few-ctas", "one-long", "odd-groups-7", "one-cta", "gqa8"]
+    ws = torch.zeros(16 << 20, dtype=torch.uint8, device="cuda")
+    for name in names * 2:
+        c, pool, q_bits, q, tables, lens, opt = _setup(name)
+        want, bound = R.attention(pool, q, tables, lens, group=c["group"], layer=c.get("layer", 0), **opt)
+        got = _attend(b2, c["dt"], pool, q_bits, tables, lens, group=c["group"], layer=c.get("layer", 0), max_ctas=c.get("max_ctas", 0),
+                      ws=ws, **dict(opt))[0]
+        _check(got, want, bound, c["dt"])
+    assert not ws[:4096].any()  # the counters
+    assert b2.device_errors() == 0
+
+
+@pytest.mark.parametrize("dt,dim,group", [(R.F16, 64, 3), (R.BF16, 128, 4)])
+def test_attention_on_any_number_of_ctas(b2, cuda, dt, dim, group):
+    rng = _rng(77)
+    lens = np.array([700, 3, 64], np.int32)
+    tables, blocks = tables_for(rng, lens)
+    pool = _filled(rng, blocks, 1, 2, dim)
+    q_bits, q = rows16(rng, dt, (3, 2 * group, dim))
+    want, bound = R.attention(pool, q, tables, lens, group=group)
+    for n in (1, 2, 5, 17, 100, 0):
+        _check(_attend(b2, dt, pool, q_bits, tables, lens, group=group, max_ctas=n)[0], want, bound, dt)
+
+
+def test_tiny_softcap_and_zero_scores(b2, cuda):
+    # x / cap overflows for every nonzero score: tanh is 1 or -1, and 0 for the zero query of head 1.
+    rng = _rng(78)
+    lens = np.array([40], np.int32)
+    tables, blocks = tables_for(rng, lens)
+    pool = _filled(rng, blocks, 1, 2, 64)
+    q_bits, q = rows16(rng, R.F16, (1, 2, 64))
+    q_bits[0, 1], q[0, 1] = 0, 0.0
+    want, bound = R.attention(pool, q, tables, lens, group=1, softcap=1e-37)
+    _check(_attend(b2, R.F16, pool, q_bits, tables, lens, group=1, softcap=1e-37)[0], want, bound, R.F16)
+    assert b2.device_errors() == 0
+
+
 # ------------------------------------------------------------------ together
 
 def _step(b2, s, stream=None):
