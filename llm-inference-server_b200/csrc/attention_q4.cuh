@@ -45,7 +45,7 @@
 //   128 sequences of 256 to 1011 tokens, 25 heads x 64            49 us, 2.9 TB/s
 //   64 sequences of 128 to 1024 tokens, 12 heads x 64             16 us, 1.7 TB/s
 // Streaming the same chunks without the arithmetic takes 68, 43, 31 and 11 us: the rest is
-// instruction issue (351 warp instructions a chunk of head_dim 128, 55 % of the issue
+// instruction issue (325 warp instructions a chunk of head_dim 128, 54 % of the issue
 // slots), and on the short calls the chain from the wait for the kernel before to the
 // first chunk (4 us) and through the merges (4 us).
 #pragma once

@@ -1573,14 +1573,14 @@ namespace {
 
 // Cluster kernels of blocks.cuh: shared bytes above the default need the opt-in.
 template <typename K, typename P>
-int launch_blocks(K kern, std::atomic<uint64_t>& smem_set, int smem, const P& prm, cudaStream_t stream, int clusters = 1) {
+int launch_blocks(K kern, std::atomic<uint64_t>& smem_set, int smem, const P& prm, cudaStream_t stream, int ctas = kMapCluster) {
     int dev = -1;
     const DeviceInfo di = device_info(&dev);
     if (dev < 0) return fail(B2_ERR_DEVICE, "no current CUDA device");
     // The limit, less the kernels' static shared memory.
     const int rc = ensure_max_smem(kern, smem_set, dev, di.max_smem_optin - 1024);
     if (rc != B2_OK) return rc;
-    return launch_pdl(kern, dim3(static_cast<unsigned>(clusters * kMapCluster)), dim3(kMapThreads), smem, stream, prm);
+    return launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kMapThreads), smem, stream, prm);
 }
 
 // The largest slot is below 2^31, and the chunk index (block, layer, head) too.
@@ -1747,16 +1747,18 @@ int b2_block_map(const B2BlockMapArgs* a, b2_stream_t stream) {
     BlockMapParams p{a->n_seqs, a->max_blocks_per_seq, a->num_blocks, a->max_rows, a->seq_lens_pre, a->new_lens,
                      a->free_list, a->free_count, a->block_tables, a->slots, a->q_start, a->seq_lens_post,
                      a->free_count_out};
-    static std::atomic<uint64_t> smem_set[2];
+    static std::atomic<uint64_t> smem_set[3];
     const int smem = 4 * (3 * a->n_seqs + 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     // One cluster maps four rows a thread in one pass, more passes take more clusters (139 k rows: 13.7 us with one, 7.4
     // with five); updates in place need a single one.
     const bool in_place = a->seq_lens_post == a->seq_lens_pre || a->free_count_out == a->free_count;
     const int passes = (a->max_rows + 4 * kMapCluster * kMapThreads - 1) / (4 * kMapCluster * kMapThreads);
-    const int clusters = in_place ? 1 : std::max(1, std::min(8, passes));
-    if (a->n_seqs <= kMapThreads) return launch_blocks(block_map_kernel<1>, smem_set[0], smem, p, s, clusters);
-    return launch_blocks(block_map_kernel<kMapPer>, smem_set[1], smem, p, s, clusters);
+    const int ctas = kMapCluster * (in_place ? 1 : std::max(1, std::min(8, passes)));
+    if (a->n_seqs <= kMapThreads && a->max_rows <= 4 * kMapThreads)
+        return launch_blocks(block_map_small_kernel, smem_set[2], smem, p, s, 1);
+    if (a->n_seqs <= kMapThreads) return launch_blocks(block_map_kernel<1>, smem_set[0], smem, p, s, ctas);
+    return launch_blocks(block_map_kernel<kMapPer>, smem_set[1], smem, p, s, ctas);
 }
 
 int b2_block_release(const B2BlockReleaseArgs* a, b2_stream_t stream) {

@@ -113,17 +113,14 @@ __device__ __forceinline__ int read_free_count(const int* p, int num_blocks, uns
 // Shared words: row[n + 1], blk[n], pre[n].  kPer: sequences to a thread, at most; small calls take the
 // kernel for one (the loops over them are unrolled, and a launch that is all latency pays for
 // every instruction it fetches: 64 sequences 6.4 -> 4.8 us).
-template <int kPer>
-__global__ void __cluster_dims__(kMapCluster, 1, 1) __launch_bounds__(kMapThreads)
-block_map_kernel(const BlockMapParams p) {
+template <int kPer, bool kCluster>
+__device__ __forceinline__ void block_map(const BlockMapParams& p) {
     extern __shared__ __align__(16) unsigned smem_u[];
     __shared__ unsigned scratch[33];
     __shared__ unsigned s_used;
     unsigned* s_row = smem_u;             // first row of sequence b
     unsigned* s_blk = s_row + p.n + 1;    // blocks needed before b; kMapRefused: b is refused
     int* s_pre = reinterpret_cast<int*>(s_blk + p.n);
-    namespace cg = cooperative_groups;
-    cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x;
     const int rank = static_cast<int>(blockIdx.x);
     pdl_launch_dependents();
@@ -197,7 +194,8 @@ block_map_kernel(const BlockMapParams p) {
     if (used != 0) atomicMax(&s_used, used);  // the same value whatever the order
     // Also the CTA's barrier: s_* are complete.  Where lengths or count are updated in place there is one
     // cluster, and every CTA has read them now.
-    cluster.sync();
+    if constexpr (kCluster) cooperative_groups::this_cluster().sync();
+    else __syncthreads();
 
     // rows, four to a thread: one binary search, one 16-byte store
     const int quads = (p.max_rows + 3) / 4;
@@ -252,6 +250,16 @@ block_map_kernel(const BlockMapParams p) {
     }
     if (err & B2_DEVERR_BLOCK_ID) flag_error(B2_DEVERR_BLOCK_ID);
 }
+
+template <int kPer>
+__global__ void __cluster_dims__(kMapCluster, 1, 1) __launch_bounds__(kMapThreads)
+block_map_kernel(const BlockMapParams p) {
+    block_map<kPer, true>(p);
+}
+
+// Up to kMapThreads sequences and 4 kMapThreads rows: one CTA, no cluster (64 sequences, one row each: 4.7 us in a
+// cluster, 4.1 so).
+__global__ void __launch_bounds__(kMapThreads) block_map_small_kernel(const BlockMapParams p) { block_map<1, false>(p); }
 
 // CTA `rank` takes a contiguous share of the sequences; the shares' totals meet
 // through distributed shared memory.  Shared words: first[share + 1], bad[share].
