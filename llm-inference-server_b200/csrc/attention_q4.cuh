@@ -23,18 +23,18 @@
 //   * Values: A = V codes transposed (16 dims x 16 tokens), B = f16(p s 2^k) per
 //     group of 32 dims; C adds up sum p s c.  The f16 rounding of p s would count
 //     with c up to 15; adding the same product with A = -8 makes it count with
-//     c - 8 instead.  sum p m is a product with
-//     A = m.  Relative to an output of the values' spread that leaves ~2^-13 rms,
-//     under the rounding of an f16 output.  The k of 2^k keeps p s in f16's
-//     normal range whatever the values' size.
+//     c - 8 instead.  sum p m is a product with A = m and B = f16(p).  Relative to
+//     an output of the values' spread that leaves 2 10^-4 rms, as much as rounding
+//     an output to f16 does.  The k of 2^k keeps p s in f16's normal range whatever
+//     the values' size.
 //   * Softmax: R_h is a reference that moves only when a score passes it by 4
 //     (p <= 16); then, or when s 2^k grows past 2^11, the accumulators are
 //     rescaled.  Sums are fp32.
 //
-// Work: the (sequence, kv head, block) chunks of the call form one list,
-// split evenly over all warps (a multiple of chunks each, contiguous).  A warp
-// streams its chunks -- each one contiguous 20 * head_dim bytes -- through its own
-// ring of shared-memory stages with cp.async.bulk, without any CTA barrier.
+// Work: a step is two chunks -- the 20 * head_dim contiguous bytes of a block and kv
+// head -- one after the other of an item (sequence, kv head).  The call's steps form one
+// list, split evenly over all warps in contiguous parts.  A warp streams its steps
+// through its own ring of shared memory with cp.async.bulk, without any CTA barrier.
 // Pieces of an item (sequence, kv head) that several warps hold meet in shared
 // memory, those of several CTAs in the workspace; the CTA that arrives last
 // merges them in CTA order, so results do not depend on timing.
@@ -497,18 +497,17 @@ __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q
     __shared__ Q4Entry s_open[2];  // items of this CTA that other CTAs hold parts of
     __shared__ int s_last[2];
     __shared__ int2 s_parts[2];  // their first CTA and number of CTAs
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane & 3, r = lane >> 2;
     __shared__ uint64_t s_bars[kQ4Warps][kQ4Slots];
     __shared__ int4 s_list[kQ4Warps][64];  // the warp's next steps: (chunk, chunk or -1, item, first block)
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, i = lane & 3, r = lane >> 2;
     const int piece_bytes = q4_piece_bytes(p.group, DH);
     constexpr int kRing = kQ4Slots * 2 * C::kBytes;
     uint8_t* ring = smem + warp * kRing;
     uint8_t* pieces = smem + kQ4Warps * kRing;
     uint64_t* bars = s_bars[warp];
-    // A piece's state: slot 0 (the warp's first chunks) has its own room, slot 1 (its last) takes the drained ring.
+    // A piece's state: slot 0 (the warp's first steps) has its own room, slot 1 (its last) takes the drained ring.
     auto piece_at = [&](int w, int slot) {
-        return reinterpret_cast<float*>(slot == 0 ? pieces + w * piece_bytes
-                                                  : smem + w * kRing);
+        return reinterpret_cast<float*>(slot == 0 ? pieces + w * piece_bytes : smem + w * kRing);
     };
     if (lane == 0) {
 #pragma unroll 1
@@ -584,7 +583,7 @@ __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q
     Q4State<DH> st;
     int item = -1, first = 0, n = 0, from_blk = 0;
     unsigned from = c0;
-    // Writes the item's result, or this warp's part of it where it holds not all of its chunks.
+    // Writes the item's result, or this warp's part of it where it holds not all of its steps.
     auto end_item = [&](unsigned upto) {
         float o[2][G][4], l[2];
         q4_finish<DH>(st, o, l);
