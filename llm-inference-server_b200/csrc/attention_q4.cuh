@@ -40,13 +40,12 @@
 // merges them in CTA order, so results do not depend on timing.
 //
 // Measured on one B200 (copy rate 6453 GB/s), a launch among others in a graph:
-//   32 sequences of 512 to 32768 tokens, 32/8 heads x 128, bf16   92 us, 4.3 TB/s
-//   61 sequences, window 4096, capped scores, same heads          59 us, 3.8 TB/s
-//   128 sequences of 256 to 1011 tokens, 25 heads x 64            49 us, 2.9 TB/s
-//   64 sequences of 128 to 1024 tokens, 12 heads x 64             16 us, 1.7 TB/s
+//   32 sequences of 512 to 32768 tokens, 32/8 heads x 128, bf16   89 us, 4.5 TB/s
+//   61 sequences, window 4096, capped scores, same heads          58 us, 3.9 TB/s
+//   128 sequences of 256 to 1011 tokens, 25 heads x 64            46 us, 3.1 TB/s
+//   64 sequences of 128 to 1024 tokens, 12 heads x 64             15 us, 1.7 TB/s
 // Streaming the same chunks without the arithmetic takes 68, 43, 31 and 11 us: the rest is
-// instruction issue (325 warp instructions a chunk of head_dim 128, 54 % of the issue
-// slots), and on the short calls the chain from the wait for the kernel before to the
+// instruction issue (300 warp instructions a chunk of head_dim 128, 52 % of the issue slots), and on the short calls the chain from the wait for the kernel before to the
 // first chunk (4 us) and through the merges (4 us).
 #pragma once
 
@@ -139,6 +138,26 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
 }
 __device__ __forceinline__ float2 half2_floats(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Two fp32 operations in one instruction (sm_100): a = a op b, elementwise, for what the two heads of a lane do
+// alike (long GQA contexts 92 -> 89 us, 25 heads x 64 49 -> 46).
+#define B2_F32X2(NAME, OP)                                                                                     \
+    __device__ __forceinline__ void NAME(float (&a)[2], float b0, float b1) {                                  \
+        asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t" OP                      \
+            ".rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"                                                 \
+            : "+f"(a[0]), "+f"(a[1])                                                                           \
+            : "f"(b0), "f"(b1));                                                                               \
+    }
+B2_F32X2(mul2, "mul")
+B2_F32X2(add2, "add")
+B2_F32X2(sub2, "sub")
+#undef B2_F32X2
+__device__ __forceinline__ void fma2(float (&a)[2], float b0, float b1, float c0, float c1) {  // a += b c
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmov.b64 z, {%4, %5};\n\t"
+        "fma.rn.f32x2 x, y, z, x;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a[0]), "+f"(a[1])
+        : "f"(b0), "f"(b1), "f"(c0), "f"(c1));
 }
 
 // N words from shared memory (volatile: they stay between the waits for a stage and its refill).
@@ -304,9 +323,10 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
                     __byte_perm(wb, wb, 0x3232), st.qb[0], st.qb[1]);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) x[2 * u + t][h] = z[2 * t + h] * 0x1p-18f;
+        for (int t = 0; t < 2; ++t) {
+            x[2 * u + t][0] = z[2 * t], x[2 * u + t][1] = z[2 * t + 1];
+            mul2(x[2 * u + t], 0x1p-18f, 0x1p-18f);
+        }
         // A product that adds to another's sum waits for it (some 20 cycles): all first ones go before all second ones.
         float c[G][4];
 #pragma unroll
@@ -320,18 +340,13 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const float sa = half2_floats(pa[g]).y, sb = half2_floats(pb[g]).y;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                x[2 * u][h] = fmaf(sa, c[g][h], x[2 * u][h]);
-                x[2 * u + 1][h] = fmaf(sb, c[g][2 + h], x[2 * u + 1][h]);
-            }
+            fma2(x[2 * u], sa, sa, c[g][0], c[g][1]);
+            fma2(x[2 * u + 1], sb, sb, c[g][2], c[g][3]);
         }
     }
     // Rounded before the reference is taken off: the largest score's weight is 1 however large it is.
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) x[t][h] *= st.sc[h];
+    for (int t = 0; t < 4; ++t) mul2(x[t], st.sc[0], st.sc[1]);
     if (__builtin_expect(p.softcap > 0.0f, 0)) {
         const float cap = p.softcap * kLog2e;
 #pragma unroll
@@ -398,12 +413,12 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
         }
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            x[t][h] = ex2_approx(x[t][h] - st.ref[h]);  // the weights from here on
-            st.l[h] += x[t][h];
-        }
+    for (int t = 0; t < 4; ++t) {
+        sub2(x[t], st.ref[0], st.ref[1]);
+        x[t][0] = ex2_approx(x[t][0]);  // the weights from here on
+        x[t][1] = ex2_approx(x[t][1]);
+        add2(st.l, x[t][0], x[t][1]);
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u) {  // sum p m: A rows = groups (rows from G on repeat them, unused)
         const uint32_t m0 = ld_word(stage[u] + at.ma), m1 = ld_word(stage[u] + at.mb);
@@ -414,9 +429,7 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
     }
     const float up = __uint_as_float(static_cast<uint32_t>(127 + st.k) << 23);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) x[t][h] *= up;
+    for (int t = 0; t < 4; ++t) mul2(x[t], up, up);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         uint32_t v[4][G / 2];  // words of product columns 2i, 2i + 1 and 8 later: groups 2w (low) and 2w + 1 (high)
@@ -428,8 +441,11 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const float sa = half2_floats(vp[2 * u][g]).y, sb = half2_floats(vp[2 * u + 1][g]).y;
-            b0[g] = transpose8x8(half2_bits(x[2 * u][0] * sa, x[2 * u][1] * sa));
-            b1[g] = transpose8x8(half2_bits(x[2 * u + 1][0] * sb, x[2 * u + 1][1] * sb));
+            float pa[2] = {x[2 * u][0], x[2 * u][1]}, pb[2] = {x[2 * u + 1][0], x[2 * u + 1][1]};
+            mul2(pa, sa, sa);
+            mul2(pb, sb, sb);
+            b0[g] = transpose8x8(half2_bits(pa[0], pa[1]));
+            b1[g] = transpose8x8(half2_bits(pb[0], pb[1]));
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -620,7 +636,7 @@ __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q
     const Q4Lane<DH> offs;
     bool alive = true;
     // The loop below is about as fast as its instructions arrive (two builds that differ only in where the kernel
-    // lies measure 92 and 98 us on long GQA contexts), so what is rare in it and in q4_step is marked, to lie apart.
+    // lies measure 89 and 96 us on long GQA contexts), so what is rare in it and in q4_step is marked, to lie apart.
     unsigned c = c0, item_end = c0;
     int blk = 0;
     while (c0 < c1) {
