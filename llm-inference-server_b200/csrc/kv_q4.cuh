@@ -62,11 +62,13 @@ __device__ __forceinline__ uint32_t q4_codes_exact(const float (&x)[8], float m,
 
 // The codes of 8 elements; rs = 1 / s, ms = -m / s.  q = x rs + ms in one fused step is off by at most 2^-22 (2 |ms| +
 // 16) from the quotient, so rounding it gives the code wherever it is further than that from a rounding
-// border, and no code needs cutting off where m's own rounding (2^-11 |m|) is under 0.45 s (`plain`).  Anything
-// else -- 0.06 % of the elements of normal bf16 rows, mostly exact ties; groups far from zero for their
-// width; saturated ones -- takes the definition.  Four codes are added up as c0 + 16 c1 + 256 c2 + 4096 c3 in
-// fp32 (exact): fp32 instructions issue at twice the integer ones' rate.
-__device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float m, float s, float rs, float ms, bool plain) {
+// border: within `limit` of an integer.  No code needs cutting off where s is a normal f16 (off by 2^-11 of itself at
+// most, which puts the range's upper end at 7.01; a subnormal s may be off by half of itself and the end
+// at 14.5) and m's own rounding (2^-11 |m|) is under 0.45 s; elsewhere limit is 0.  What is not within it -- 0.06 %
+// of the elements of normal bf16 rows, mostly exact ties; groups far from zero for their width; steps
+// below 2^-14; saturated groups -- takes the definition.  Four codes are added up as c0 + 16 c1 + 256 c2 + 4096 c3 in fp32 (exact): fp32 instructions
+// issue at twice the integer ones' rate.
+__device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float m, float s, float rs, float ms, float limit) {
     constexpr float kMagic = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer, ties to even
     float far = 0.0f, packed[2];
 #pragma unroll
@@ -80,7 +82,7 @@ __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float m, float
             packed[w] = fmaf(k, static_cast<float>(1 << (4 * e)), packed[w]);
         }
     }
-    if (plain && far < 0.49999f - fabsf(ms) * 0x1p-21f)
+    if (far < limit)
         return __byte_perm(__float_as_uint(packed[0]), __float_as_uint(packed[1]), 0x5410);
     return q4_codes_exact(x, m, s, rs);
 }
@@ -172,7 +174,8 @@ __global__ void __launch_bounds__(256) kv_append_q4_kernel(const KvQ4Params p, i
         const float s = __half2float(sh);
         const __half mh = __float2half_rn(fmaf(8.0f, s, lo));
         const float m = __half2float(mh), rs = __frcp_rn(s), ms = -m * rs;
-        const bool plain = !saturated && fabsf(ms) * 0x1p-11f < 0.45f;  // also false for s = 0
+        const bool plain = !saturated && s >= 0x1p-14f && fabsf(ms) * 0x1p-11f < 0.45f;
+        const float limit = plain ? 0.49999f - fabsf(ms) * 0x1p-21f : 0.0f;
         const int t = slot % kBlockTokens;
         uint8_t* chunk = p.pool + static_cast<size_t>(slot / kBlockTokens) * block_bytes +
                          (static_cast<size_t>(p.layer_idx) * p.n_kv_head + h) * C::kBytes;
@@ -182,7 +185,7 @@ __global__ void __launch_bounds__(256) kv_append_q4_kernel(const KvQ4Params p, i
         for (int i = 0; i < 4; ++i) {
             float x[8];
             unpack16<T>(raw[i], x);
-            const uint32_t codes = s > 0.0f ? q4_codes(x, m, s, rs, ms, plain) : 0x88888888u;
+            const uint32_t codes = s > 0.0f ? q4_codes(x, m, s, rs, ms, limit) : 0x88888888u;
             if (!is_v) {
                 *reinterpret_cast<uint32_t*>(chunk + C::k_word(t, i, g)) = codes;
             } else {
