@@ -380,8 +380,9 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int g = 0; g < G; g += 2) s_top = __vimax3_u32(s_top, vp[t][g], vp[t][g + 1]);
+    // The difference, not top - 4 > ref: from 2^26 on that sum rounds, to ref itself for a score 8 above it.
     // (no short circuit: branches here cost long GQA contexts 98 against 93 us)
-    const bool moves = (top[0] - 4.0f > st.ref[0]) | (top[1] - 4.0f > st.ref[1]) | (s_top >= st.s_limit);
+    const bool moves = (top[0] - st.ref[0] > 4.0f) | (top[1] - st.ref[1] > 4.0f) | (s_top >= st.s_limit);
     if (__builtin_expect(__any_sync(0xffffffffu, moves), 0)) {
         s_top = 0;
 #pragma unroll

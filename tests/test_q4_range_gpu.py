@@ -1,7 +1,13 @@
-"""The 4-bit paged KV pool where its numbers reach far: steps below f16's normal range.
+"""The 4-bit paged KV pool where its numbers reach far: steps below f16's normal range, score caps of any size, long
+contexts with one dominant key, values of very different sizes, scores near the end of fp32's precision.
 
 Tolerances (set from arithmetic before the first run):
-  * the bytes an append writes: equal.
+  * the bytes an append writes: equal;
+  * attention: with w the exact weights, S and M the largest step and |middle| a group of 32 dims meets and n keys,
+      (2^-11 + 2 e) sum w (8 s + |m|)  +  n (2^-30 S + 2^-36 M)  +  2^-20 max w max (8 s + |m|)
+    where 2^-11 covers the rounding of weight times step and of weight to f16, n 2^-30 S and n 2^-36 M what weights far
+    below the largest lose to f16's smallest number, and e the error of a score: 2^-18 (sum of the magnitudes of its
+    products, + 1) and, under a cap, 2^-19 of the capped score; plus half a step of the output's type.
 """
 from __future__ import annotations
 
@@ -10,9 +16,37 @@ import pytest
 
 import q4_ref as R
 from test_kernels_gpu import ints_dev, to_dev
-from test_q4_gpu import _rng, _torch
+from test_q4_gpu import _attend, _check, _filled, _rng, _torch, rows16, tables_for
 
 pytestmark = pytest.mark.gpu
+
+
+def _want(pool, q, tables, lens, *, group, softcap=0.0, scale=0.0):
+    """(out, bound) in float64.  Slots that a table names repeatedly are computed once."""
+    batch, heads, dim = q.shape
+    scale = scale or 1.0 / np.sqrt(dim)
+    out, bound = np.zeros_like(q), np.zeros_like(q)
+    for b in range(batch):
+        n = int(lens[b])
+        j = np.arange(n)
+        slots, times = np.unique(tables[b][j // 16].astype(np.int64) * 16 + j % 16, return_counts=True)
+        k, v, ks, km, vs, vm = pool.rows(slots, 0)
+        for h in range(heads):
+            hk = h // group
+            x = scale * (k[:, hk] @ q[b, h])
+            mag = scale * ((8 * ks[:, hk] + np.abs(km[:, hk])).repeat(32, -1) @ np.abs(q[b, h]))
+            err = 2.0 ** -18 * (mag.max() + 1.0)
+            if softcap:
+                x = softcap * np.tanh(x / softcap)
+                err += 2.0 ** -19 * np.abs(x).max()
+            w = np.exp(x - x.max()) * times
+            top = 1.0 / w.sum()
+            w *= top
+            out[b, h] = w @ v[:, hk]
+            each = (8 * vs[:, hk] + np.abs(vm[:, hk])).repeat(32, -1)
+            lost = n * (2.0 ** -30 * vs[:, hk].max(0) + 2.0 ** -36 * np.abs(vm[:, hk]).max(0)).repeat(32)
+            bound[b, h] = (2.0 ** -11 + 2 * err) * (w @ each) + lost + 2.0 ** -20 * top * each.max(0)
+    return out, bound
 
 
 # ------------------------------------------------------------------ append
@@ -56,3 +90,57 @@ def test_append_of_groups_with_subnormal_steps(b2, cuda, dt, dim):
         pool.put(r, 0, x[r, 0], x[r, 1])
     assert np.array_equal(dev.cpu().numpy(), pool.b)
     assert b2.device_errors() == 0
+
+
+# ------------------------------------------------------------------ attention
+
+def test_scores_of_any_size_choose_the_largest(b2, cuda):
+    """Queries up to 2^110: where the largest score leads by more than its rounding, the output is that key's value."""
+    rng = _rng(91)
+    lens = np.array([300, 33, 5], np.int32)
+    tables, blocks = tables_for(rng, lens)
+    pool = _filled(rng, blocks, 1, 2, 64)
+    clear = 0
+    for top in (20, 24, 26, 27, 28, 30, 60, 100, 108):
+        q_bits, q = rows16(rng, R.BF16, (3, 4, 64), 2.0 ** (top - 2))
+        got = _attend(b2, R.BF16, pool, q_bits, tables, lens, group=2)[0]
+        assert np.all(np.isfinite(got))
+        for b in range(3):
+            j = np.arange(lens[b])
+            k, v, ks, km, vs, vm = pool.rows(tables[b][j // 16].astype(np.int64) * 16 + j % 16, 0)
+            for h in range(4):
+                x = k[:, h // 2] @ q[b, h] / 8.0
+                mag = ((8 * ks[:, h // 2] + np.abs(km[:, h // 2])).repeat(32, -1) @ np.abs(q[b, h])).max() / 8.0
+                first, second = np.sort(x)[::-1][:2]
+                if first - second <= 2.0 ** -17 * mag + 60.0:  # a lead of 60 leaves the others e^-60
+                    continue
+                clear += 1
+                i = int(np.argmax(x))
+                want = v[i, h // 2]
+                each = (8 * vs[i, h // 2] + np.abs(vm[i, h // 2])).repeat(32)
+                assert np.all(np.abs(got[b, h] - want) <= 2.0 ** -11 * each + np.abs(want) * 2.0 ** -7)
+    assert clear > 60
+
+
+def test_scores_a_rounding_step_apart(b2, cuda):
+    """Scores of 2^26 to 2^27 (in log2 units), where fp32 holds multiples of 8: in each warp the second step's are about one step above
+    the first's, and the steps of its values 2^6 times the first's."""
+    torch = _torch()
+    dim, heads, batch = 64, 1, 128  # (one head: a head whose reference moves takes the others along)
+    rng = _rng(92)
+    pool = R.Pool(4, 1, 1, dim, np.zeros(4 * 20 * dim))
+    small = (rng.standard_normal((1, dim))).astype(np.float16).astype(np.float64)
+    for s in range(64):
+        k = np.ones((1, dim))  # a step of 0: exact
+        k[0, 32:] = 1.0 if s < 32 else 2.0
+        pool.put(s, 0, k, small if s < 32 else small * 64.0)
+    q = np.zeros((batch, heads, dim))
+    q[..., 0] = 2.0 ** 28 * rng.uniform(1.4, 2.7, size=(batch, heads))  # x = (q0 + q1 or 2 q1) / 8 log2 e
+    q[..., 32] = 8.0 * 8.0 / np.log2(np.e) * rng.uniform(0.8, 1.5, size=(batch, heads))
+    q_bits = R.O.round_to(R.BF16, q.astype(np.float32).ravel()).reshape(q.shape)
+    tables = np.tile(np.tile(np.arange(4, dtype=np.int32), 4), (batch, 1))
+    got = _attend(b2, R.BF16, pool, q_bits, tables, np.full(batch, 256, np.int32), group=1, out_dtype=torch.float32, max_ctas=128)[0]
+    v = pool.rows(np.arange(64), 0)[1][:, 0]
+    lo, hi = v.min(0), v.max(0)
+    slack = 2.0 ** -10 * (hi - lo + np.abs(hi) + np.abs(lo))
+    assert np.all(np.isfinite(got)) and np.all(got >= lo - slack) and np.all(got <= hi + slack)
