@@ -29,7 +29,9 @@
 //     the values' size.
 //   * Softmax: R_h is a reference that moves only when a score passes it by 4
 //     (p <= 16); then, or when s 2^k grows past 2^11, the accumulators are
-//     rescaled.  Sums are fp32.
+//     rescaled.  Sums are fp32.  Weights are held as 2^11 p (up to 2^15): f16(p) would
+//     drop what lies 25 binary orders below the largest, which in long contexts adds
+//     up (3 % of the middles' sum at 2^20 such keys); 2^11 p drops n 2^-36 at most.
 //
 // Work: a step is two chunks -- the 20 * head_dim contiguous bytes of a block and kv
 // head -- one after the other of an item (sequence, kv head).  The call's steps form one
@@ -84,6 +86,7 @@ constexpr int kQ4Slots = 2;
 constexpr int kQ4MaxCtas = 1024;  // the workspace's counters: as many whatever the call's shape, so that calls of different shapes may share one
 constexpr int kQ4MaxGroup = 8;
 constexpr int kQ4FewParts = 4;  // parts of an item that a CTA merges straight from L2
+constexpr int kQ4Weight = 11;   // weights are 2^kQ4Weight p
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Bytes of one piece's state in shared memory: [group][head_dim] sums, [group] (R, l).
@@ -182,7 +185,7 @@ struct Q4State {
     static constexpr int G = DH / 32;
     float acc[G][2][4];  // [group][dims 4r+0,1 | 4r+2,3][(dim, head 2i), (dim, 2i+1), (dim+1, 2i), (dim+1, 2i+1)]
     float tz[4];         // row g: sum p m of group g
-    float ref[2], l[2];  // heads 2i, 2i+1; l is this lane's share
+    float ref[2], l[2];  // heads 2i, 2i+1: the reference less kQ4Weight, and this lane's share of the weights
     int k;
     uint32_t s_limit;    // param words from here on need a smaller k
     uint32_t qf[G][4];   // B fragments of head r
@@ -380,9 +383,10 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
     for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int g = 0; g < G; g += 2) s_top = __vimax3_u32(s_top, vp[t][g], vp[t][g + 1]);
-    // The difference, not top - 4 > ref: from 2^26 on that sum rounds, to ref itself for a score 8 above it.
+    // The difference, not top - c > ref: from 2^26 on that sum rounds, to ref itself for a score 8 above it.
     // (no short circuit: branches here cost long GQA contexts 98 against 93 us)
-    const bool moves = (top[0] - st.ref[0] > 4.0f) | (top[1] - st.ref[1] > 4.0f) | (s_top >= st.s_limit);
+    constexpr float kMost = kQ4Weight + 4;
+    const bool moves = (top[0] - st.ref[0] > kMost) | (top[1] - st.ref[1] > kMost) | (s_top >= st.s_limit);
     if (__builtin_expect(__any_sync(0xffffffffu, moves), 0)) {
         s_top = 0;
 #pragma unroll
@@ -399,7 +403,7 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
-            const float ref = fmaxf(st.ref[h], top[h]);
+            const float ref = fmaxf(st.ref[h], __fadd_ru(top[h], -kQ4Weight));  // up: the weights stay below 2^15
             const float f = ex2_approx(st.ref[h] - ref);
             st.ref[h] = ref;
             st.l[h] *= f;
@@ -416,7 +420,7 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         sub2(x[t], st.ref[0], st.ref[1]);
-        x[t][0] = ex2_approx(x[t][0]);  // the weights from here on
+        x[t][0] = ex2_approx(x[t][0]);  // 2^kQ4Weight p from here on
         x[t][1] = ex2_approx(x[t][1]);
         add2(st.l, x[t][0], x[t][1]);
     }
@@ -428,7 +432,7 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
         const uint32_t b1 = transpose8x8(half2_bits(x[2 * u + 1][0], x[2 * u + 1][1]));
         mma_f16(st.tz, __byte_perm(m0, m1, 0x5410), 0, __byte_perm(m2, m3, 0x5410), 0, b0, b1);
     }
-    const float up = __uint_as_float(static_cast<uint32_t>(127 + st.k) << 23);
+    const float up = __uint_as_float(static_cast<uint32_t>(127 - kQ4Weight + st.k) << 23);
 #pragma unroll
     for (int t = 0; t < 4; ++t) mul2(x[t], up, up);
 #pragma unroll
@@ -470,7 +474,7 @@ template <int DH>
 __device__ __forceinline__ void q4_finish(Q4State<DH>& st, float (&out)[2][DH / 32][4], float (&l)[2]) {
     constexpr int G = DH / 32;
     const int i = threadIdx.x & 3;
-    const float f = __uint_as_float(static_cast<uint32_t>(127 + 24 - st.k) << 23);
+    const float f = __uint_as_float(static_cast<uint32_t>(127 + 24 + kQ4Weight - st.k) << 23);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         l[h] = st.l[h];

@@ -94,6 +94,30 @@ def test_append_of_groups_with_subnormal_steps(b2, cuda, dt, dim):
 
 # ------------------------------------------------------------------ attention
 
+@pytest.mark.parametrize("n", [131072, 1 << 20])
+@pytest.mark.parametrize("spread", [0.0])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_keys_far_below_a_peak_keep_their_mass(b2, cuda, dim, spread, n):
+    # The warps of one CTA take a quarter of the keys each; each quarter has one key 25.4 binary orders above the others.
+    torch = _torch()
+    pool = R.Pool(2, 1, 1, dim, np.zeros(2 * 20 * dim))
+    d = np.arange(dim)
+    plain, peak = np.zeros((1, dim)), np.zeros((1, dim))
+    peak[0, 0] = 17.6
+    some = (1.0 + spread * np.sin(d))[None].astype(np.float16).astype(np.float64)
+    for s in range(32):
+        pool.put(s, 0, peak if s == 3 else plain, np.zeros((1, dim)) if s == 3 else some)
+    q = np.zeros((1, 1, dim))
+    q[0, 0, 0] = np.sqrt(128.0) if dim == 128 else 8.0
+    q_bits = R.O.round_to(R.F16, q.astype(np.float32).ravel()).reshape(q.shape)
+    q = R.widen(R.F16, q_bits)
+    tables = np.ones((1, n // 16), np.int32)
+    tables[0, ::n // 64] = 0
+    want, bound = _want(pool, q, tables, [n], group=1)
+    got = _attend(b2, R.F16, pool, q_bits, tables, np.array([n], np.int32), group=1, out_dtype=torch.float32, max_ctas=1)[0]
+    _check(got, want, bound, R.F16, True)
+
+
 def test_scores_of_any_size_choose_the_largest(b2, cuda):
     """Queries up to 2^110: where the largest score leads by more than its rounding, the output is that key's value."""
     rng = _rng(91)
