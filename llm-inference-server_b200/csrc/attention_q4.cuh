@@ -20,15 +20,16 @@
 //     product whose columns are m and s and whose B is Q in two f16 parts.
 //     q is scaled by a power of two to at most 2^9, so its f16 form is exact
 //     down to 2^-23 of the row's largest element.
-//   * Values: A = V codes transposed (16 dims x 16 tokens), B = f16(p s 2^k) per
+//   * Values: A = V codes transposed (16 dims x 16 tokens), B = f16(p s 2^k), k per
 //     group of 32 dims; C adds up sum p s c.  The f16 rounding of p s would count
 //     with c up to 15; adding the same product with A = -8 makes it count with
 //     c - 8 instead.  sum p m is a product with A = m and B = f16(p).  Relative to
 //     an output of the values' spread that leaves 2 10^-4 rms, as much as rounding
-//     an output to f16 does.  The k of 2^k keeps p s in f16's normal range whatever
-//     the values' size.
+//     an output to f16 does.  k follows the largest step S that the warp has met in the group:
+//     2^8 <= S 2^k < 2^11 (above 2^-1 if S is subnormal).  So f16 rounds a p s above 2^-22 S to
+//     its 11 bits, and a smaller one to a multiple of 2^-32 S: 2^-30 S of output a key at most.
 //   * Softmax: R_h is a reference that moves only when a score passes it by 4
-//     (p <= 16); then, or when s 2^k grows past 2^11, the accumulators are
+//     (p <= 16); then, or when an s 2^k grows past 2^11, the accumulators are
 //     rescaled.  Sums are fp32.  Weights are held as 2^11 p (up to 2^15): f16(p) would
 //     drop what lies 25 binary orders below the largest, which in long contexts adds
 //     up (3 % of the middles' sum at 2^20 such keys); 2^11 p drops n 2^-36 at most.
@@ -186,16 +187,30 @@ struct Q4State {
     float acc[G][2][4];  // [group][dims 4r+0,1 | 4r+2,3][(dim, head 2i), (dim, 2i+1), (dim+1, 2i), (dim+1, 2i+1)]
     float tz[4];         // row g: sum p m of group g
     float ref[2], l[2];  // heads 2i, 2i+1: the reference less kQ4Weight, and this lane's share of the weights
-    int k;
-    uint32_t s_limit;    // param words from here on need a smaller k
+    uint32_t scale[G];   // high half: steps from here on need a smaller k; low half: 2^(k - kQ4Weight) as f16
     uint32_t qf[G][4];   // B fragments of head r
     uint32_t qb[2];      // B fragment of head r: Q_i 2^-6 as (high, low) f16 parts, and -8 times them
     float sc[2];         // S -> score (log2 units; with a cap: the exponent's argument)
     float slope[2];      // log2 units
 };
 
-__device__ __forceinline__ uint32_t q4_s_limit(int k) {
-    return static_cast<uint32_t>(min((26 - k) << 10, 0xffff)) << 16;  // words with s >= 2^(11 - k)
+// The scale word of a k from -7 to 25: s 2^k < 2^11 below the limit (an f16's exponent bits, 26 - k), and the factor
+// exactly (a subnormal f16 below k = -3).  A step that equals the limit and passes it by its middle's bits alone is
+// taken as below it: 2^11, with weights of up to 2^4 still in f16's range.
+__device__ __forceinline__ uint32_t q4_scale(int k) {
+    const int e = k - kQ4Weight;
+    return static_cast<uint32_t>(26 - k) << 26 | static_cast<uint32_t>(e >= -14 ? (e + 15) << 10 : 1 << (e + 24));
+}
+__device__ __forceinline__ int q4_scale_k(uint32_t w) { return 26 - static_cast<int>(w >> 26); }
+
+// s 2^(k - kQ4Weight), exactly: s in the high half of w, the factor in the low half of scale.
+__device__ __forceinline__ float q4_scaled_step(uint32_t w, uint32_t scale) {
+    float x;
+    asm("{\n\t.reg .f16 m, s, f, limit;\n\tmov.b32 {m, s}, %1;\n\tmov.b32 {f, limit}, %2;\n\t"
+        "fma.rn.f32.f16 %0, s, f, %3;\n\t}"
+        : "=f"(x)
+        : "r"(w), "r"(scale), "f"(0.0f));
+    return x;
 }
 
 // Loads the query heads of item (b, hk) and clears the sums.
@@ -252,8 +267,8 @@ __device__ __forceinline__ void q4_start(const Q4AttnParams& p, int b, int hk, Q
         st.ref[h] = -FLT_MAX;
         st.l[h] = 0.0f;
     }
-    st.k = 18;
-    st.s_limit = q4_s_limit(18);
+#pragma unroll
+    for (int g = 0; g < G; ++g) st.scale[g] = q4_scale(25);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         st.tz[c] = 0.0f;
@@ -378,27 +393,26 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
     float top[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(x[0][h], x[1][h]), fmaxf(x[2][h], x[3][h]));
-    uint32_t s_top = 0;
+    bool grows = false;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int g = 0; g < G; g += 2) s_top = __vimax3_u32(s_top, vp[t][g], vp[t][g + 1]);
+    for (int g = 0; g < G; ++g) grows |= max(__vimax3_u32(vp[0][g], vp[1][g], vp[2][g]), vp[3][g]) >= st.scale[g];
     // The difference, not top - c > ref: from 2^26 on that sum rounds, to ref itself for a score 8 above it.
     // (no short circuit: branches here cost long GQA contexts 98 against 93 us)
     constexpr float kMost = kQ4Weight + 4;
-    const bool moves = (top[0] - st.ref[0] > kMost) | (top[1] - st.ref[1] > kMost) | (s_top >= st.s_limit);
+    const bool moves = (top[0] - st.ref[0] > kMost) | (top[1] - st.ref[1] > kMost) | grows;
     if (__builtin_expect(__any_sync(0xffffffffu, moves), 0)) {
-        s_top = 0;
+        float by[G];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int g = 0; g < G; ++g) {
+            uint32_t s_top = 0;
 #pragma unroll
-            for (int g = 0; g < G; ++g)  // NaN and infinite steps do not count
+            for (int t = 0; t < 4; ++t)  // NaN and infinite steps do not count
                 if (vp[t][g] < 0x7c000000u) s_top = max(s_top, vp[t][g]);
-        s_top = __reduce_max_sync(0xffffffffu, s_top);
-        const int k = min(st.k, 18 - static_cast<int>(s_top >> 26));  // s 2^k < 2^4
-        const float by = __uint_as_float(static_cast<uint32_t>(127 + k - st.k) << 23);
-        st.k = k;
-        st.s_limit = q4_s_limit(k);
+            s_top = __reduce_max_sync(0xffffffffu, s_top);
+            const int old = q4_scale_k(st.scale[g]), k = min(old, 23 - static_cast<int>(s_top >> 26));  // s 2^k < 2^9
+            by[g] = __uint_as_float(static_cast<uint32_t>(127 + k - old) << 23);
+            st.scale[g] = q4_scale(k);
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -412,8 +426,8 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
             for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    st.acc[g][t][h] *= f * by;
-                    st.acc[g][t][2 + h] *= f * by;
+                    st.acc[g][t][h] *= f * by[g];
+                    st.acc[g][t][2 + h] *= f * by[g];
                 }
         }
     }
@@ -432,9 +446,6 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
         const uint32_t b1 = transpose8x8(half2_bits(x[2 * u + 1][0], x[2 * u + 1][1]));
         mma_f16(st.tz, __byte_perm(m0, m1, 0x5410), 0, __byte_perm(m2, m3, 0x5410), 0, b0, b1);
     }
-    const float up = __uint_as_float(static_cast<uint32_t>(127 - kQ4Weight + st.k) << 23);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) mul2(x[t], up, up);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         uint32_t v[4][G / 2];  // words of product columns 2i, 2i + 1 and 8 later: groups 2w (low) and 2w + 1 (high)
@@ -445,7 +456,7 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
         uint32_t b0[G], b1[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            const float sa = half2_floats(vp[2 * u][g]).y, sb = half2_floats(vp[2 * u + 1][g]).y;
+            const float sa = q4_scaled_step(vp[2 * u][g], st.scale[g]), sb = q4_scaled_step(vp[2 * u + 1][g], st.scale[g]);
             float pa[2] = {x[2 * u][0], x[2 * u][1]}, pb[2] = {x[2 * u + 1][0], x[2 * u + 1][1]};
             mul2(pa, sa, sa);
             mul2(pb, sb, sb);
@@ -474,7 +485,6 @@ template <int DH>
 __device__ __forceinline__ void q4_finish(Q4State<DH>& st, float (&out)[2][DH / 32][4], float (&l)[2]) {
     constexpr int G = DH / 32;
     const int i = threadIdx.x & 3;
-    const float f = __uint_as_float(static_cast<uint32_t>(127 + 24 + kQ4Weight - st.k) << 23);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         l[h] = st.l[h];
@@ -483,6 +493,7 @@ __device__ __forceinline__ void q4_finish(Q4State<DH>& st, float (&out)[2][DH / 
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             const float c = __shfl_sync(0xffffffffu, st.tz[h], 4 * g + i);
+            const float f = __uint_as_float(static_cast<uint32_t>(127 + 24 + kQ4Weight - q4_scale_k(st.scale[g])) << 23);
             out[h][g][0] = fmaf(st.acc[g][0][h], f, c);
             out[h][g][1] = fmaf(st.acc[g][0][2 + h], f * 0.0625f, c);
             out[h][g][2] = fmaf(st.acc[g][1][h], f, c);

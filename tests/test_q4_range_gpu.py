@@ -95,7 +95,7 @@ def test_append_of_groups_with_subnormal_steps(b2, cuda, dt, dim):
 # ------------------------------------------------------------------ attention
 
 @pytest.mark.parametrize("n", [131072, 1 << 20])
-@pytest.mark.parametrize("spread", [0.0])
+@pytest.mark.parametrize("spread", [0.0, 1.0])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_keys_far_below_a_peak_keep_their_mass(b2, cuda, dim, spread, n):
     # The warps of one CTA take a quarter of the keys each; each quarter has one key 25.4 binary orders above the others.
@@ -115,6 +115,39 @@ def test_keys_far_below_a_peak_keep_their_mass(b2, cuda, dim, spread, n):
     tables[0, ::n // 64] = 0
     want, bound = _want(pool, q, tables, [n], group=1)
     got = _attend(b2, R.F16, pool, q_bits, tables, np.array([n], np.int32), group=1, out_dtype=torch.float32, max_ctas=1)[0]
+    _check(got, want, bound, R.F16, True)
+
+
+@pytest.mark.parametrize("ratio", [10, 14, 18, 22])
+@pytest.mark.parametrize("dt,dim,group", [(R.F16, 64, 2), (R.BF16, 128, 4)])
+def test_groups_of_dims_of_different_sizes(b2, cuda, dt, dim, group, ratio):
+    torch = _torch()
+    rng = _rng(ratio + dim)
+    lens = np.array([500, 40, 1], np.int32)
+    tables, blocks = tables_for(rng, lens)
+    spread = np.where(np.arange(dim) // 32 == 1, 2.0 ** (ratio - 10), 2.0 ** -10)
+    pool = _filled(rng, blocks, 1, 2, dim, v_spread=spread)
+    q_bits, q = rows16(rng, dt, (3, 2 * group, dim), 3.0)
+    want, bound = _want(pool, q, tables, lens, group=group)
+    got = _attend(b2, dt, pool, q_bits, tables, lens, group=group, out_dtype=torch.float32)[0]
+    _check(got, want, bound, dt, True)
+
+
+@pytest.mark.parametrize("ratio", [8, 12, 16])
+@pytest.mark.parametrize("at", [0, 150, 299])
+def test_one_key_with_huge_values_and_no_weight(b2, cuda, ratio, at):
+    torch = _torch()
+    rng = _rng(ratio + at)
+    dim, n = 64, 300
+    tables, blocks = tables_for(rng, [n])
+    pool = _filled(rng, blocks, 1, 1, dim, v_spread=2.0 ** -3)
+    q_bits, q = rows16(rng, R.F16, (1, 2, dim))
+    q_bits[0, 1], q[0, 1] = q_bits[0, 0], q[0, 0]
+    k = -5.0 * np.sign(q[0, :1])
+    v = rng.standard_normal((1, dim)) * 2.0 ** (ratio - 3)
+    pool.put(int(tables[0, at // 16]) * 16 + at % 16, 0, k, v.astype(np.float16).astype(np.float64))
+    want, bound = _want(pool, q, tables, [n], group=2)
+    got = _attend(b2, R.F16, pool, q_bits, tables, np.array([n], np.int32), group=2, out_dtype=torch.float32)[0]
     _check(got, want, bound, R.F16, True)
 
 
