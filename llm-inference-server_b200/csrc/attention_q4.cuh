@@ -73,7 +73,7 @@ struct Q4AttnParams {
     float* ws_acc;       // [2 grid][group][head_dim]
     int batch, n_head, n_kv_head, group, mbps, layer_idx, n_layer, num_blocks, window;
     unsigned kv_mul, kv_shift;  // n / n_kv_head = n * kv_mul >> kv_shift for n < 2^31
-    float scale, softcap;
+    float scale, cap, cap_inv;  // the score cap in log2 units (0: none) and its reciprocal, both finite
 };
 
 constexpr int kQ4Warps = 4;
@@ -164,6 +164,13 @@ __device__ __forceinline__ void fma2(float (&a)[2], float b0, float b1, float c0
         : "f"(b0), "f"(b1), "f"(c0), "f"(c1));
 }
 
+__device__ __forceinline__ void mul2_add(float (&a)[2], float b0, float b1, float c) {  // a = a b + c
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmov.b64 z, {%4, %4};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a[0]), "+f"(a[1])
+        : "f"(b0), "f"(b1), "f"(c));
+}
+
 // N words from shared memory (volatile: they stay between the waits for a stage and its refill).
 template <int N>
 __device__ __forceinline__ void ld_words(uint32_t at, uint32_t (&w)[N]) {
@@ -190,7 +197,7 @@ struct Q4State {
     uint32_t scale[G];   // high half: steps from here on need a smaller k; low half: 2^(k - kQ4Weight) as f16
     uint32_t qf[G][4];   // B fragments of head r
     uint32_t qb[2];      // B fragment of head r: Q_i 2^-6 as (high, low) f16 parts, and -8 times them
-    float sc[2];         // S -> score (log2 units; with a cap: the exponent's argument)
+    float sc[2];         // S -> score in log2 units
     float slope[2];      // log2 units
 };
 
@@ -255,10 +262,9 @@ __device__ __forceinline__ void q4_start(const Q4AttnParams& p, int b, int hk, Q
     const float high = __half2float(__float2half_rn(sum_i));
     st.qb[0] = half2_bits(high, sum_i - high);
     st.qb[1] = half2_bits(-8.0f * high, -8.0f * (sum_i - high));
-    // score = S 2^24 / norm * scale; the cap's argument is 2 score / cap (exp of it in log2 units)
-    const float unit = p.softcap > 0.0f ? 2.0f * kLog2e * p.scale / p.softcap : kLog2e * p.scale;
-    // (finite, so that S = 0 stays 0 under the smallest caps)
-    const float sc = fminf(fmaxf(unit * 0x1p24f * __uint_as_float(static_cast<uint32_t>(127 - up) << 23), -FLT_MAX), FLT_MAX);
+    // score = S 2^24 / norm * scale (finite, so that S = 0 stays 0)
+    const float unit = kLog2e * p.scale * 0x1p24f * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+    const float sc = fminf(fmaxf(unit, -FLT_MAX), FLT_MAX);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int src = 4 * (2 * i + h);
@@ -365,13 +371,37 @@ __device__ __forceinline__ void q4_step(const Q4AttnParams& p, const Q4Lane<DH>&
     // Rounded before the reference is taken off: the largest score's weight is 1 however large it is.
 #pragma unroll
     for (int t = 0; t < 4; ++t) mul2(x[t], st.sc[0], st.sc[1]);
-    if (__builtin_expect(p.softcap > 0.0f, 0)) {
-        const float cap = p.softcap * kLog2e;
+    if (__builtin_expect(p.cap > 0.0f, 0)) {
+        // cap tanh(y), y = x / cap.  Up to 1/2: x (tanh(y) / y), with tanh(y) / y - 1 = y^2 R(y^2), R the minimax cubic
+        // (2^-26 relative); beyond: cap (1 - 2 / (1 + e^2y)), whose 2^-22 of the cap is 2^-21 of the score there and would
+        // be any share of a smaller one.
+        float capped[4][2], top = 0.0f;
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 4; ++t) {
+            float y[2] = {x[t][0], x[t][1]};
+            mul2(y, p.cap_inv, p.cap_inv);
+            top = fmaxf(top, fmaxf(fabsf(y[0]), fabsf(y[1])));
+            mul2(y, y[0], y[1]);
+            float r[2] = {0.01724149f, 0.01724149f};
+            mul2_add(r, y[0], y[1], -0.05304549f);
+            mul2_add(r, y[0], y[1], 0.13325879f);
+            mul2_add(r, y[0], y[1], -0.33333144f);
+            mul2(r, y[0], y[1]);
+            capped[t][0] = x[t][0], capped[t][1] = x[t][1];
+            fma2(capped[t], x[t][0], x[t][1], r[0], r[1]);
+        }
+        if (__any_sync(0xffffffffu, top > 0.5f)) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)  // tanh(y) = 1 - 2 / (1 + e^2y): 2^-23 absolute, to be multiplied by the cap
-                x[t][h] = cap - __fdividef(2.0f * cap, 1.0f + ex2_approx(x[t][h]));
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float y = x[t][h] * p.cap_inv;
+                    const float w = __fdividef(2.0f, 1.0f + ex2_approx(2.0f * kLog2e * y));
+                    if (fabsf(y) > 0.5f) capped[t][h] = fmaf(-p.cap, w, p.cap);
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t][0] = capped[t][0], x[t][1] = capped[t][1];
     }
     if (__builtin_expect(p.slopes != nullptr, 0)) {
         const float d = static_cast<float>(pos + at.tk - (n - 1));

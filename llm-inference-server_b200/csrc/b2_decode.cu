@@ -1824,7 +1824,9 @@ int b2_paged_attention_q4(const B2PagedAttnQ4Args* a, void* workspace, size_t wo
     p.num_blocks = a->num_blocks;
     p.window = a->window;
     p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt(static_cast<float>(a->head_dim));
-    p.softcap = a->softcap;
+    constexpr double kMost = 3.4028234663852886e38;  // FLT_MAX
+    p.cap = static_cast<float>(std::min(a->softcap * 1.4426950408889634, kMost));
+    p.cap_inv = a->softcap > 0.0f ? static_cast<float>(std::min(0.6931471805599453 / a->softcap, kMost)) : 0.0f;
     unsigned up = 0;
     while ((1ull << up) < static_cast<unsigned long long>(a->n_kv_head)) ++up;
     p.kv_shift = 31 + up;

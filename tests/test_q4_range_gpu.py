@@ -94,6 +94,21 @@ def test_append_of_groups_with_subnormal_steps(b2, cuda, dt, dim):
 
 # ------------------------------------------------------------------ attention
 
+@pytest.mark.parametrize("cap", [0.25, 3.0, 30.0, 1e2, 1e3, 1e5, 1e7, 1e30, 3e38])
+@pytest.mark.parametrize("dt,dim,group", [(R.F16, 64, 1), (R.BF16, 128, 4)])
+def test_a_cap_of_any_size_keeps_the_scores(b2, cuda, dt, dim, group, cap):
+    torch = _torch()
+    rng = _rng(int(np.log2(cap)) + 50)
+    lens = np.array([300, 1, 77, 32], np.int32)
+    tables, blocks = tables_for(rng, lens)
+    pool = _filled(rng, blocks, 1, 2, dim)
+    q_bits, q = rows16(rng, dt, (4, 2 * group, dim), 5.0)
+    want, bound = _want(pool, q, tables, lens, group=group, softcap=cap)
+    got = _attend(b2, dt, pool, q_bits, tables, lens, group=group, softcap=cap, out_dtype=torch.float32)[0]
+    _check(got, want, bound, dt, True)
+    assert b2.device_errors() == 0
+
+
 @pytest.mark.parametrize("n", [131072, 1 << 20])
 @pytest.mark.parametrize("spread", [0.0, 1.0])
 @pytest.mark.parametrize("dim", [64, 128])
