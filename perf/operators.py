@@ -340,7 +340,9 @@ def _run_own(s):
     plan = s.get("plan")
     if plan is None:  # argument structs and workspaces, which a program keeps
         if op == "map":
-            plan = b2.block_map_args(s["tables"], s["pre"], s["free"], s["count"], s["slots"], new_lens=s["new"], q_start=s["start"],
+            free = s["free"].new_zeros(s["blocks"])  # a pool's list has room for every block's id
+            free[:s["free"].numel()] = s["free"]
+            plan = b2.block_map_args(s["tables"], s["pre"], free, s["count"], s["slots"], new_lens=s["new"], q_start=s["start"],
                                      seq_lens_post=s["post"], free_count_out=s["count_out"], num_blocks=s["blocks"])
         elif op == "release":
             plan = b2.block_release_args(s["tables"], s["lens"], s["gone"], s["free"], s["count"], seq_lens_out=s["lens_out"],
