@@ -370,10 +370,11 @@ def _q4_pool(pool, num_blocks, n_layer, n_kv_head, head_dim):
 
 def block_map_args(block_tables, seq_lens_pre, free_list, free_count, slots, *, num_blocks, new_lens=None, q_start=None,
                    seq_lens_post=None, free_count_out=None) -> BlockMapArgs:
-    """Arguments of block_map.  free_count_out=None updates free_count in place."""
+    """Arguments of block_map.  free_list has room for every block's id (num_blocks entries); free_count_out=None updates
+    free_count in place."""
     n, mbps = block_tables.shape
     for name, t, c in (("block_tables", block_tables, None), ("seq_lens_pre", seq_lens_pre, n), ("slots", slots, None),
-                       ("free_list", free_list, 1), ("free_count", free_count, 1), ("new_lens", new_lens, n),
+                       ("free_list", free_list, num_blocks), ("free_count", free_count, 1), ("new_lens", new_lens, n),
                        ("q_start", q_start, n), ("seq_lens_post", seq_lens_post, n), ("free_count_out", free_count_out, 1)):
         if t is not None:
             _int32(name, t, c)
