@@ -184,14 +184,24 @@ def _ptr(t) -> int | None:
 _current = None
 
 
+def _current_calls():
+    """(raw current stream of a device, current device): what torch.cuda.current_stream().cuda_stream and
+    torch.cuda.current_device() give, without making a Stream object each call."""
+    global _current
+    if _current is None:
+        from torch import _C
+        _current = (_C._cuda_getCurrentRawStream, _C._cuda_getDevice)
+    return _current
+
+
+def _current_device() -> int:
+    return _current_calls()[1]()
+
+
 def _stream(stream) -> int | None:
     if stream is None:
-        # what torch.cuda.current_stream().cuda_stream is, without making a Stream object each call
-        global _current
-        if _current is None:
-            from torch import _C
-            _current = (_C._cuda_getCurrentRawStream, _C._cuda_getDevice)
-        return _current[0](_current[1]())
+        raw, device = _current_calls()
+        return raw(device())
     return stream if isinstance(stream, int) else stream.cuda_stream
 
 
@@ -352,7 +362,17 @@ def _on_device(args, *tensors):
         if t is not None and not (t.is_cuda and t.device.index == torch.cuda.current_device()):
             raise ValueError(f"a tensor is on {t.device}, not on the current CUDA device")
     args.tensors = tensors
+    args.device = torch.cuda.current_device()
     return args
+
+
+def _launch_stream(args, stream):
+    """The stream of a launch with args: the launch goes to the current device, which must be that of args' tensors."""
+    raw = _stream(stream)
+    device = getattr(args, "device", None)  # (a struct filled by hand has none)
+    if device is not None and device != _current_device():
+        raise ValueError(f"the arguments' tensors are on cuda:{device}, not on the current CUDA device")
+    return raw
 
 
 def _int32(name, t, count=None):
@@ -390,7 +410,7 @@ def block_map(args: BlockMapArgs, stream=None) -> None:
     """Blocks for each sequence's new rows from the device free list, and the
     slot of every row (b2_block_map; the reference's BlockPool allocates on the
     host, kv_cache.h:16-57)."""
-    _check(load().b2_block_map(ctypes.byref(args), _stream(stream)))
+    _check(load().b2_block_map(ctypes.byref(args), _launch_stream(args, stream)))
 
 
 def block_release_args(block_tables, seq_lens, release, free_list, free_count, *, num_blocks, seq_lens_out=None,
@@ -410,7 +430,7 @@ def block_release_args(block_tables, seq_lens, release, free_list, free_count, *
 
 def block_release(args: BlockReleaseArgs, stream=None) -> None:
     """The blocks of released sequences go back on the device free list (b2_block_release)."""
-    _check(load().b2_block_release(ctypes.byref(args), _stream(stream)))
+    _check(load().b2_block_release(ctypes.byref(args), _launch_stream(args, stream)))
 
 
 def kv_q4_pool(num_blocks, *, n_layer, n_kv_head, head_dim, device=None):
@@ -439,12 +459,12 @@ def kv_q4_args(kv_pool, k, v, slots, *, n_kv_head, head_dim, layer_idx, n_layer,
 
 def kv_append_q4(args: KvQ4Args, stream=None) -> None:
     """Rows of k and v, quantised to 4 bits, into their slots of the pool (b2_kv_append_q4)."""
-    _check(load().b2_kv_append_q4(ctypes.byref(args), _stream(stream)))
+    _check(load().b2_kv_append_q4(ctypes.byref(args), _launch_stream(args, stream)))
 
 
 def kv_gather_q4(args: KvQ4Args, stream=None) -> None:
     """The values of the pool's slots into rows of k and v (b2_kv_gather_q4)."""
-    _check(load().b2_kv_gather_q4(ctypes.byref(args), _stream(stream)))
+    _check(load().b2_kv_gather_q4(ctypes.byref(args), _launch_stream(args, stream)))
 
 
 def attn_q4_args(q, kv_pool, block_tables, seq_lens, out, *, n_head, n_kv_head, head_dim, layer_idx, n_layer, num_blocks,
@@ -481,4 +501,4 @@ def attention_q4_workspace(args: PagedAttnQ4Args, device=None):
 
 def paged_attention_q4(args: PagedAttnQ4Args, workspace, stream=None) -> None:
     """Decode attention over the 4-bit pool (b2_paged_attention_q4)."""
-    _check(load().b2_paged_attention_q4(ctypes.byref(args), workspace.data_ptr(), workspace.numel(), _stream(stream)))
+    _check(load().b2_paged_attention_q4(ctypes.byref(args), workspace.data_ptr(), workspace.numel(), _launch_stream(args, stream)))

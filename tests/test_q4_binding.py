@@ -16,3 +16,21 @@ def test_block_map_refuses_a_free_list_shorter_than_the_pool(b2):
             b2.block_map_args(_ints(-1, -1).view(1, 2), _ints(0), _ints(*range(n)), _ints(n), _ints(0), num_blocks=4)
     with pytest.raises(ValueError, match="device"):  # long enough: the next check
         b2.block_map_args(_ints(-1, -1).view(1, 2), _ints(0), _ints(0, 1, 2, 3), _ints(3), _ints(0), num_blocks=4)
+
+
+def test_launches_refuse_arguments_of_another_device(b2, monkeypatch):
+    device = 0
+    monkeypatch.setattr(b2, "_current", (lambda d: 0, lambda: device))
+    calls = [(b2.block_map, b2.BlockMapArgs()), (b2.block_release, b2.BlockReleaseArgs()), (b2.kv_append_q4, b2.KvQ4Args(dtype=b2.F16)),
+             (b2.kv_gather_q4, b2.KvQ4Args(dtype=b2.F16)),
+             (lambda a, stream=None: b2.paged_attention_q4(a, torch.empty(16, dtype=torch.uint8), stream), b2.PagedAttnQ4Args())]
+    for call, args in calls:
+        args.device = 1
+        for stream in (None, 0):
+            with pytest.raises(ValueError, match="cuda:1"):
+                call(args, stream)
+        device = 1
+        with pytest.raises((b2.B2Error, ValueError)) as e:  # the right device: the next check
+            call(args)
+        assert "cuda:1" not in str(e.value)
+        device = 0
