@@ -500,5 +500,9 @@ def attention_q4_workspace(args: PagedAttnQ4Args, device=None):
 
 
 def paged_attention_q4(args: PagedAttnQ4Args, workspace, stream=None) -> None:
-    """Decode attention over the 4-bit pool (b2_paged_attention_q4)."""
-    _check(load().b2_paged_attention_q4(ctypes.byref(args), workspace.data_ptr(), workspace.numel(), _launch_stream(args, stream)))
+    """Decode attention over the 4-bit pool (b2_paged_attention_q4).  workspace: attention_q4_workspace's, or any zeroed
+    contiguous tensor of that many bytes on the arguments' device."""
+    raw = _launch_stream(args, stream)
+    if not workspace.is_cuda or workspace.get_device() != getattr(args, "device", workspace.get_device()) or not workspace.is_contiguous():
+        raise ValueError("the workspace must be a contiguous tensor on the arguments' CUDA device")
+    _check(load().b2_paged_attention_q4(ctypes.byref(args), workspace.data_ptr(), workspace.numel() * workspace.element_size(), raw))

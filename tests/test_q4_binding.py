@@ -34,3 +34,37 @@ def test_launches_refuse_arguments_of_another_device(b2, monkeypatch):
             call(args)
         assert "cuda:1" not in str(e.value)
         device = 0
+
+
+def test_attention_refuses_a_workspace_that_the_kernel_cannot_use(b2, monkeypatch):
+    monkeypatch.setattr(b2, "_current", (lambda d: 0, lambda: 0))
+
+    class OnGpu:  # what the binding asks of a tensor
+        is_cuda = True
+
+        def __init__(self, device=0, contiguous=True):
+            self.device_index, self.contiguous = device, contiguous
+
+        def get_device(self):
+            return self.device_index
+
+        def is_contiguous(self):
+            return self.contiguous
+
+        def data_ptr(self):
+            return 16
+
+        def numel(self):
+            return 0
+
+        def element_size(self):
+            return 1
+
+    args = b2.PagedAttnQ4Args()
+    args.device = 0
+    # host memory, another device's, an expanded tensor whose bytes it does not have
+    for ws in (torch.zeros(1 << 20, dtype=torch.uint8), OnGpu(device=1), OnGpu(contiguous=False)):
+        with pytest.raises(ValueError, match="workspace"):
+            b2.paged_attention_q4(args, ws)
+    with pytest.raises(b2.B2Error):  # the library's own checks come next
+        b2.paged_attention_q4(args, OnGpu())
