@@ -382,6 +382,11 @@ def _int32(name, t, count=None):
     return t
 
 
+def _row_stride(t, width):
+    """Elements between rows of width elements; a single row's own stride means nothing and may be any."""
+    return t.stride(0) if t.shape[0] > 1 else width
+
+
 def _q4_pool(pool, num_blocks, n_layer, n_kv_head, head_dim):
     need = load().b2_kv_q4_pool_bytes(num_blocks, n_layer, n_kv_head, head_dim)
     if need and (not pool.is_contiguous() or pool.numel() * pool.element_size() < need):
@@ -448,11 +453,12 @@ def kv_q4_args(kv_pool, k, v, slots, *, n_kv_head, head_dim, layer_idx, n_layer,
     rows = slots.numel()
     _int32("slots", slots)
     _q4_pool(kv_pool, num_blocks, n_layer, n_kv_head, head_dim)
+    width = n_kv_head * head_dim
     for t in (k, v):
-        if t.shape[0] != rows or t[0:1].numel() != (n_kv_head * head_dim if rows else 0) or t.dtype != k.dtype \
-                or (rows > 0 and not t[0].is_contiguous()) or t.stride(0) != k.stride(0):
+        if t.shape[0] != rows or t[0:1].numel() != (width if rows else 0) or t.dtype != k.dtype \
+                or (rows > 0 and not t[0].is_contiguous()) or _row_stride(t, width) != _row_stride(k, width):
             raise ValueError("k and v must have slots.numel() rows of n_kv_head * head_dim contiguous elements, one dtype and row stride")
-    a = KvQ4Args(dtype_code(k.dtype), _ptr(kv_pool), _ptr(k), _ptr(v), k.stride(0), _ptr(slots), rows, n_kv_head, head_dim,
+    a = KvQ4Args(dtype_code(k.dtype), _ptr(kv_pool), _ptr(k), _ptr(v), _row_stride(k, width), _ptr(slots), rows, n_kv_head, head_dim,
                  layer_idx, n_layer, num_blocks)
     return _on_device(a, kv_pool, k, v, slots)
 
@@ -483,7 +489,7 @@ def attn_q4_args(q, kv_pool, block_tables, seq_lens, out, *, n_head, n_kv_head, 
     if alibi_slopes is not None and (alibi_slopes.dtype != torch.float32 or alibi_slopes.numel() != n_head
                                      or not alibi_slopes.is_contiguous()):
         raise ValueError("alibi_slopes must be float32 [n_head]")
-    a = PagedAttnQ4Args(dtype_code(q.dtype), dtype_code(out.dtype), _ptr(q), q.stride(0), _ptr(kv_pool),
+    a = PagedAttnQ4Args(dtype_code(q.dtype), dtype_code(out.dtype), _ptr(q), _row_stride(q, n_head * head_dim), _ptr(kv_pool),
                         _ptr(block_tables), _ptr(seq_lens), _ptr(key_starts), _ptr(alibi_slopes), _ptr(out), batch,
                         n_head, n_kv_head, head_dim, mbps, layer_idx, n_layer, num_blocks, scale, softcap, window,
                         max_ctas)

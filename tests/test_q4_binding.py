@@ -68,3 +68,25 @@ def test_attention_refuses_a_workspace_that_the_kernel_cannot_use(b2, monkeypatc
             b2.paged_attention_q4(args, ws)
     with pytest.raises(b2.B2Error):  # the library's own checks come next
         b2.paged_attention_q4(args, OnGpu())
+
+
+def test_a_single_row_may_have_any_row_stride(b2, monkeypatch):
+    # A tensor's stride over one row means nothing: [heads, 1, dim] transposed has one head's.
+    monkeypatch.setattr(b2, "_on_device", lambda args, *tensors: args)
+    heads, dim = 4, 64
+    kv = dict(n_kv_head=heads, head_dim=dim, layer_idx=0, n_layer=1, num_blocks=2)
+    pool = torch.zeros(2, 1, heads, 20 * dim, dtype=torch.uint8)
+    one = torch.zeros(heads, 1, dim, dtype=torch.float16).transpose(0, 1)
+    wide = torch.zeros(1, 3 * heads * dim, dtype=torch.float16)[:, :heads * dim]
+    assert one.shape == (1, heads, dim) and one.stride(0) == dim
+    for k, v in ((one, one), (one, wide), (wide, one), (wide, wide), (one.expand(1, heads, dim), one)):
+        assert b2.kv_q4_args(pool, k, v, _ints(3), **kv).row_stride == heads * dim
+    two = torch.zeros(2, 3, heads, dim, dtype=torch.float16)
+    assert b2.kv_q4_args(pool, two[:, 0], two[:, 1], _ints(3, 4), **kv).row_stride == 3 * heads * dim
+    with pytest.raises(ValueError):  # two rows: the strides count
+        b2.kv_q4_args(pool, two[:, 0], two[:, 0].contiguous(), _ints(3, 4), **kv)
+    shape = dict(n_head=heads, **kv)
+    out = torch.zeros(1, heads, dim, dtype=torch.float16)
+    for q in (one, wide):
+        assert b2.attn_q4_args(q, pool, _ints(0).view(1, 1), _ints(5), out, **shape).q_row_stride == heads * dim
+    assert b2.attn_q4_args(two[:, 0], pool, _ints(0, 1).view(2, 1), _ints(5, 5), torch.zeros(2, heads, dim).half(), **shape).q_row_stride == 3 * heads * dim
