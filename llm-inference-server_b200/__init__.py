@@ -194,13 +194,9 @@ def _current_calls():
     return _current
 
 
-def _current_device() -> int:
-    return _current_calls()[1]()
-
-
 def _stream(stream) -> int | None:
     if stream is None:
-        raw, device = _current_calls()
+        raw, device = _current or _current_calls()
         return raw(device())
     return stream if isinstance(stream, int) else stream.cuda_stream
 
@@ -368,11 +364,11 @@ def _on_device(args, *tensors):
 
 def _launch_stream(args, stream):
     """The stream of a launch with args: the launch goes to the current device, which must be that of args' tensors."""
-    raw = _stream(stream)
-    device = getattr(args, "device", None)  # (a struct filled by hand has none)
-    if device is not None and device != _current_device():
-        raise ValueError(f"the arguments' tensors are on cuda:{device}, not on the current CUDA device")
-    return raw
+    raw, current = _current or _current_calls()
+    device = current()
+    if getattr(args, "device", device) != device:  # (a struct filled by hand has none)
+        raise ValueError(f"the arguments' tensors are on cuda:{args.device}, not on the current CUDA device")
+    return raw(device) if stream is None else _stream(stream)
 
 
 def _int32(name, t, count=None):
@@ -509,6 +505,6 @@ def paged_attention_q4(args: PagedAttnQ4Args, workspace, stream=None) -> None:
     """Decode attention over the 4-bit pool (b2_paged_attention_q4).  workspace: attention_q4_workspace's, or any zeroed
     contiguous tensor of that many bytes on the arguments' device."""
     raw = _launch_stream(args, stream)
-    if not workspace.is_cuda or workspace.get_device() != getattr(args, "device", workspace.get_device()) or not workspace.is_contiguous():
-        raise ValueError("the workspace must be a contiguous tensor on the arguments' CUDA device")
-    _check(load().b2_paged_attention_q4(ctypes.byref(args), workspace.data_ptr(), workspace.numel() * workspace.element_size(), raw))
+    if workspace.get_device() != _current[1]() or not workspace.is_contiguous():  # (-1: in host memory)
+        raise ValueError("the workspace must be a contiguous tensor on the current CUDA device")
+    _check(load().b2_paged_attention_q4(ctypes.byref(args), workspace.data_ptr(), workspace.nbytes, raw))

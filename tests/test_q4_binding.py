@@ -40,8 +40,6 @@ def test_attention_refuses_a_workspace_that_the_kernel_cannot_use(b2, monkeypatc
     monkeypatch.setattr(b2, "_current", (lambda d: 0, lambda: 0))
 
     class OnGpu:  # what the binding asks of a tensor
-        is_cuda = True
-
         def __init__(self, device=0, contiguous=True):
             self.device_index, self.contiguous = device, contiguous
 
@@ -54,11 +52,7 @@ def test_attention_refuses_a_workspace_that_the_kernel_cannot_use(b2, monkeypatc
         def data_ptr(self):
             return 16
 
-        def numel(self):
-            return 0
-
-        def element_size(self):
-            return 1
+        nbytes = 0
 
     args = b2.PagedAttnQ4Args()
     args.device = 0
