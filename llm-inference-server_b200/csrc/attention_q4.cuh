@@ -262,8 +262,9 @@ __device__ __forceinline__ void q4_start(const Q4AttnParams& p, int b, int hk, Q
     const float high = __half2float(__float2half_rn(sum_i));
     st.qb[0] = half2_bits(high, sum_i - high);
     st.qb[1] = half2_bits(-8.0f * high, -8.0f * (sum_i - high));
-    // score = S 2^24 / norm * scale (finite, so that S = 0 stays 0)
-    const float unit = kLog2e * p.scale * 0x1p24f * __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+    // score = S 2^24 / norm * scale (finite, so that S = 0 stays 0); 1 / norm first, whose size is the opposite of a scale's
+    // that gives scores in range
+    const float unit = kLog2e * p.scale * __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * 0x1p24f;
     const float sc = fminf(fmaxf(unit, -FLT_MAX), FLT_MAX);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {

@@ -216,3 +216,18 @@ def test_scores_a_rounding_step_apart(b2, cuda):
     lo, hi = v.min(0), v.max(0)
     slack = 2.0 ** -10 * (hi - lo + np.abs(hi) + np.abs(lo))
     assert np.all(np.isfinite(got)) and np.all(got >= lo - slack) and np.all(got <= hi + slack)
+
+
+@pytest.mark.parametrize("power", [-110, -60, 60, 112])
+def test_scale_and_queries_of_opposite_size(b2, cuda, power):
+    """scale 2^power and queries of 2^-power: the same scores, and the same bits, as with neither (powers of two are exact)."""
+    rng = _rng(5)
+    lens = np.array([100, 33], np.int32)
+    tables, blocks = tables_for(rng, lens)
+    pool = _filled(rng, blocks, 1, 2, 64)
+    q_bits, q = rows16(rng, R.BF16, (2, 4, 64))
+    want, bound = _want(pool, q, tables, lens, group=2, scale=0.25)
+    plain = _attend(b2, R.BF16, pool, q_bits, tables, lens, group=2, scale=0.25)[0]
+    _check(plain, want, bound, R.BF16)
+    far = R.O.round_to(R.BF16, (q * 2.0 ** -power).astype(np.float32).ravel()).reshape(q.shape)
+    assert np.array_equal(_attend(b2, R.BF16, pool, far, tables, lens, group=2, scale=0.25 * 2.0 ** power)[0], plain)
