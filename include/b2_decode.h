@@ -500,7 +500,8 @@ B2_API int b2_lm_head_argmax(const B2LmHeadArgmaxArgs* args, b2_stream_t stream)
  *
  * seq_lens_post may be seq_lens_pre and free_count_out may be free_count
  * (in place); no other two arrays may overlap.  n_seqs <= B2_MAP_MAX_SEQS,
- * slots 16-byte aligned.  One launch of one thread-block cluster. */
+ * slots 16-byte aligned.  One launch; into separate outputs a call of many rows
+ * takes more of the GPU than in place. */
 #define B2_MAP_MAX_SEQS 16384
 
 typedef struct B2BlockMapArgs {
@@ -557,9 +558,11 @@ B2_API int b2_block_release(const B2BlockReleaseArgs* args, b2_stream_t stream);
  * element:
  *   s = f16((max - min) / 15),  m = f16(min + 8 s),
  *   c = clamp(round_to_nearest_even((x - m) / s) + 8, 0, 15)   (8 where s = 0),
- * and the element reads back as s * (c - 8) + m.  x is clamped to +-65504
- * first; a group that holds a NaN or an infinity stores NaN for s and m and
- * reads back as NaN.
+ * in fp32, and the element reads back as s * (c - 8) + m.  x is clamped to
+ * +-65504 first; a group that holds a NaN or an infinity stores NaN for s and m
+ * and reads back as NaN.  A group that spans f16's whole range can read back
+ * beyond it (-65504 .. 65504: s rounds up to 8736 and the top code stands for
+ * 65536), which is an infinity in F16 rows; the attention uses the value.
  *
  * Layout: [block][layer][n_kv_head] chunks of 20 * head_dim bytes, each 16
  * token positions of one kv head; with G = head_dim / 32,
@@ -610,7 +613,10 @@ B2_API int b2_kv_gather_q4(const B2KvQ4Args* args, b2_stream_t stream);
  * key_starts masks the keys in front of the query's own document (or a
  * left-padded batch's padding).  A sequence without visible keys gets zeros.
  * q and out F16 or BF16 (out also F32); any n_head / n_kv_head from 1 to 8.
- * |q| up to 2^110: beyond, scores overflow to NaN.
+ * |q| up to 2^110: beyond, scores overflow to NaN.  Weights times steps are
+ * rounded to f16 for the tensor cores (2^-11 relative; 2^-30 of the largest step
+ * of their group of 32 dims where that is more): an output of the values' spread
+ * is off by 2e-4 of it (rms).  Sums are fp32.
  * A seq_len beyond max_blocks_per_seq * 16 or below 0 is clamped
  * (B2_DEVERR_SEQ_LEN), a block id outside the pool is clamped
  * (B2_DEVERR_BLOCK_ID).

@@ -42,14 +42,17 @@
 // memory, those of several CTAs in the workspace; the CTA that arrives last
 // merges them in CTA order, so results do not depend on timing.
 //
-// Measured on one B200 (copy rate 6453 GB/s), a launch among others in a graph:
-//   32 sequences of 512 to 32768 tokens, 32/8 heads x 128, bf16   89 us, 4.5 TB/s
+// Measured on one B200 (copy rate 6453 GB/s), a launch among others in a graph of a few ms at 1965 MHz:
+//   32 sequences of 512 to 32768 tokens, 32/8 heads x 128, bf16   90 us, 4.4 TB/s
 //   61 sequences, window 4096, capped scores, same heads          58 us, 3.9 TB/s
-//   128 sequences of 256 to 1011 tokens, 25 heads x 64            46 us, 3.1 TB/s
-//   64 sequences of 128 to 1024 tokens, 12 heads x 64             15 us, 1.7 TB/s
-// Streaming the same chunks without the arithmetic takes 68, 43, 31 and 11 us: the rest is
-// instruction issue (300 warp instructions a chunk of head_dim 128, 52 % of the issue slots), and on the short calls the chain from the wait for the kernel before to the
-// first chunk (4 us) and through the merges (4 us).
+//   128 sequences of 256 to 1011 tokens, 25 heads x 64            47 us, 3.0 TB/s
+//   64 sequences of 128 to 1024 tokens, 12 heads x 64             16 us, 1.7 TB/s
+// (Run for seconds, the first one takes 97 us: at the 1000 W limit the clock falls to 1840 MHz.)  Streaming the same
+// chunks without the arithmetic takes 68, 42, 29 and 9 us.  The rest is the chain of dependent instructions in a
+// step with three warps a scheduler to hide it: 308 warp instructions a chunk of head_dim 128 fill half
+// of the issue slots; warps wait for results of fixed latency and for the tensor pipe (34 % active).  On the
+// short calls it is the chain from the wait for the kernel before to the first chunk (4 us) and through the
+// merges (4 us).
 #pragma once
 
 #include <cfloat>
@@ -145,7 +148,7 @@ __device__ __forceinline__ float2 half2_floats(uint32_t w) {
 }
 
 // Two fp32 operations in one instruction (sm_100): a = a op b, elementwise, for what the two heads of a lane do
-// alike (long GQA contexts 92 -> 89 us, 25 heads x 64 49 -> 46).
+// alike (long GQA contexts 94.0 -> 90.1 us, 25 heads x 64 48.0 -> 46.8, the same in four layouts of the module).
 #define B2_F32X2(NAME, OP)                                                                                     \
     __device__ __forceinline__ void NAME(float (&a)[2], float b0, float b1) {                                  \
         asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t" OP                      \
@@ -682,8 +685,7 @@ __global__ void __launch_bounds__(kQ4Threads, q4_ctas_per_sm(DH)) paged_decode_q
     };
     const Q4Lane<DH> offs;
     bool alive = true;
-    // The loop below is about as fast as its instructions arrive (two builds that differ only in where the kernel
-    // lies measure 89 and 96 us on long GQA contexts), so what is rare in it and in q4_step is marked, to lie apart.
+    // What is rare in the loop below and in q4_step is marked, to lie apart from the instructions of every step.
     unsigned c = c0, item_end = c0;
     int blk = 0;
     while (c0 < c1) {

@@ -4,13 +4,14 @@
 // Two prefix sums over the sequences carry both operators: rows (or blocks to
 // give back) before sequence b, and blocks needed before sequence b.  What
 // bounds them is latency -- a launch, a chain of dependent loads, two scans -- not
-// the few hundred KB they move, so each is one launch, of thread-block clusters:
-// every CTA reads all lengths and scans them for itself (n <= 16384 values, a
-// few L2 lines a thread) and then writes its share of the rows.  Only
-// free_count and the lengths may be updated in place; then there is one cluster,
-// every CTA of which has read them before its barrier, and they are written
-// after it.  Into separate outputs the map of many rows takes more clusters (512
-// prompts, 139 k rows: 13.7 us with one, 7.4 with five).
+// the few hundred KB they move, so each is one launch.  Map: every CTA reads all lengths
+// and scans them for itself (n <= 16384 values, a few L2 lines a thread) and then
+// writes its share of the rows; small calls take one CTA, others clusters of
+// eight.  Only free_count and the lengths may be updated in place; then there is
+// one cluster, every CTA of which has read them before its barrier, and they are
+// written after it.  Into separate outputs the map of many rows takes more clusters
+// (512 prompts, 139 k rows, in a graph: 13.7 us in place, 6.2 to 6.8 with five).  Release:
+// one cluster, whose CTAs take a share of the sequences each and meet their totals.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -258,7 +259,7 @@ block_map_kernel(const BlockMapParams p) {
 }
 
 // Up to kMapThreads sequences and 4 kMapThreads rows: one CTA, no cluster (64 sequences, one row each: 4.7 us in a
-// cluster, 4.1 so).
+// cluster, 4.1 to 4.4 so).
 __global__ void __launch_bounds__(kMapThreads) block_map_small_kernel(const BlockMapParams p) { block_map<1, false>(p); }
 
 // CTA `rank` takes a contiguous share of the sequences; the shares' totals meet

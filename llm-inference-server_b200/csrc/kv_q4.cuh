@@ -5,9 +5,8 @@
 // codes c in 0..15; an element is s (c - 8) + m.  Codes are taken against the
 // rounded s and m, so an element inside the group's range is off by at most s / 2
 // plus what the two roundings move the range's ends by.  Everything is computed in
-// fp32: with 16-bit inputs x - m is a short sum and (x - m) / s is at least
-// 2^-12 (in steps) away from a rounding border it does not hit, so the fp32
-// quotient rounds to the code the exact quotient rounds to.
+// fp32, which decides the code where (x - m) / s lies within fp32's rounding of a border
+// (an element 2^24 times smaller than m that would tip a tie does not count).
 //
 // The m half sits low and the s half high in a 32-bit word: s >= 0, so words
 // compare as their steps do.
@@ -125,8 +124,10 @@ __device__ __forceinline__ void q4_values(uint32_t codes, uint32_t w, float (&x)
 
 // Quantising: a thread takes a whole group of 32 (64 bytes), so that what is per group -- extremes, step,
 // middle, their conversions -- is worked out once and no lanes have to agree.  2 bytes read and 0.625
-// written an element; what bounds it is instruction issue, about 11 an element (with four lanes to a
-// group: 25).  16384 rows of 8 heads x 128: 43 us with four lanes to a group, 24 us so (3.6 TB/s).
+// written an element.  16384 rows of 8 heads x 128: 43 us with four lanes to a group, 23 us so (3.8 TB/s;
+// floor 13.6).  Two things share the time: 16.5 instructions an element fill 71 % of the issue slots,
+// and a thread's four loads are waited for at once (the largest stall; 5 CTAs an SM hide part of it).  The loads,
+// 64 bytes apart, and the 2- and 4-byte stores take 2 and 2.8 times the sectors, in L1 and L2; DRAM sees each byte once.
 template <typename T, int DH>
 __global__ void __launch_bounds__(256) kv_append_q4_kernel(const KvQ4Params p, int rows_per_cta) {
     using C = Q4Chunk<DH>;
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(256) kv_append_q4_kernel(const KvQ4Params p, i
 
 // Reading back: a CTA takes kRows rows, a thread 8 neighbouring elements (16 bytes) of K or of V in each.  What
 // does not depend on the row is worked out once, and the arithmetic stays off the integer and conversion
-// pipes: 65531 rows of 8 heads x 128 took 127 us with one row a thread, 70 us with four, and take 66 us
+// pipes: 65531 rows of 8 heads x 128 took 127 us with one row a thread, 70 us with four, and take 66 us in a graph
 // (5.3 TB/s) without conversions.
 template <typename T, int DH, int kRows>
 __global__ void __launch_bounds__(256) kv_gather_q4_kernel(const KvQ4Params p) {
