@@ -231,3 +231,24 @@ def test_scale_and_queries_of_opposite_size(b2, cuda, power):
     _check(plain, want, bound, R.BF16)
     far = R.O.round_to(R.BF16, (q * 2.0 ** -power).astype(np.float32).ravel()).reshape(q.shape)
     assert np.array_equal(_attend(b2, R.BF16, pool, far, tables, lens, group=2, scale=0.25 * 2.0 ** power)[0], plain)
+
+
+@pytest.mark.parametrize("size", [65504.0, 30000.0, 1e-3, 1e-5, 3e-7])
+@pytest.mark.parametrize("dt,dim,group", [(R.F16, 64, 2), (R.BF16, 128, 3)])
+def test_values_at_the_ends_of_f16s_range(b2, cuda, dt, dim, group, size):
+    """Steps of up to 8736 and down to 2^-24 (below 2^-14, f16's products of a weight and a step end at 2^-45 instead of 2^-30 of the largest)."""
+    torch = _torch()
+    rng = _rng(int(-np.log(size)) + 60)
+    lens = np.array([100, 37], np.int32)
+    tables, blocks = tables_for(rng, lens)
+    pool = _filled(rng, blocks, 1, 2, dim)
+    v = (rng.uniform(-size, size, size=(blocks * 16, 2, dim))).astype(np.float16).astype(np.float64)
+    for s in range(blocks * 16):
+        k_half = pool.b[s // 16, 0, :, :10 * dim].copy()
+        pool.put(s, 0, v[s], v[s])
+        pool.b[s // 16, 0, :, :10 * dim] = k_half  # V alone
+    q_bits, q = rows16(rng, dt, (2, 2 * group, dim), 4.0)
+    want, bound = _want(pool, q, tables, lens, group=group)
+    got = _attend(b2, dt, pool, q_bits, tables, lens, group=group, out_dtype=torch.float32)[0]
+    _check(got, want, bound + 100 * 2.0 ** -45, dt, True)
+    assert b2.device_errors() == 0
