@@ -92,6 +92,35 @@ def test_append_of_groups_with_subnormal_steps(b2, cuda, dt, dim):
     assert b2.device_errors() == 0
 
 
+@pytest.mark.parametrize("dt", [R.F16, R.BF16])
+def test_append_of_any_finite_bits_follows_the_format_in_fp32(b2, cuda, dt):
+    """Random bit patterns: elements up to 2^40 apart in one group, saturated ones, ties that fp32 decides.  The format restated in numpy's fp32."""
+    torch = _torch()
+    rng = _rng(7 + dt)
+    rows, heads, dim = 2000, 2, 64
+    bits = rng.integers(0, 65536, size=(rows, 2, heads, dim)).astype(np.uint16)
+    top = 0x7C00 if dt == R.F16 else 0x7F80
+    bits = np.where((bits & top) == top, bits & 0x83FF, bits).astype(np.uint16)  # finite
+    x = np.clip(R.widen(dt, bits), -65504.0, 65504.0).astype(np.float32).reshape(rows, 2, heads, 2, 32)
+    lo, hi = x.min(-1), x.max(-1)
+    s = ((hi - lo) / np.float32(15)).astype(np.float16)
+    m = (np.float32(8) * s.astype(np.float32) + lo).astype(np.float16)
+    s32, m32 = s.astype(np.float32)[..., None], m.astype(np.float32)[..., None]
+    c = np.where(s32 > 0, np.rint(np.clip((x - m32) / np.where(s32 > 0, s32, np.float32(1)), -8, 7)), 0)
+    want = (c.astype(np.float64) * s32 + m32).reshape(rows, 2, heads, dim)
+    pool = R.Pool(-(-rows // 16), 1, heads, dim, np.zeros(-(-rows // 16) * heads * 20 * dim))
+    dev = torch.from_numpy(pool.b).cuda()
+    kv = to_dev(dt, bits)
+    b2.kv_append_q4(b2.kv_q4_args(dev, kv[:, 0], kv[:, 1], ints_dev(np.arange(rows)), n_kv_head=heads, head_dim=dim, layer_idx=0,
+                                  n_layer=1, num_blocks=pool.b.shape[0]))
+    pool.b[:] = dev.cpu().numpy()
+    k, v, ks, km, vs, vm = pool.rows(np.arange(rows), 0)
+    for i, (got, steps, middles) in enumerate(((k, ks, km), (v, vs, vm))):
+        assert np.array_equal(steps, s[:, i].astype(np.float64)) and np.array_equal(middles, m[:, i].astype(np.float64))
+        assert np.array_equal(got, want[:, i])
+    assert b2.device_errors() == 0
+
+
 # ------------------------------------------------------------------ attention
 
 @pytest.mark.parametrize("cap", [0.25, 3.0, 30.0, 1e2, 1e3, 1e5, 1e7, 1e30, 3e38])
