@@ -616,7 +616,8 @@ B2_API int b2_kv_gather_q4(const B2KvQ4Args* args, b2_stream_t stream);
  * |q| up to 2^110: beyond, scores overflow to NaN.  Weights times steps are
  * rounded to f16 for the tensor cores (2^-11 relative; 2^-30 of the largest step
  * of their group of 32 dims where that is more): an output of the values' spread
- * is off by 2e-4 of it (rms).  Sums are fp32.
+ * is off by 2e-4 of it (rms).  Elements of q are kept to 2^-29 of their row's
+ * largest.  Sums are fp32.
  * A seq_len beyond max_blocks_per_seq * 16 or below 0 is clamped
  * (B2_DEVERR_SEQ_LEN), a block id outside the pool is clamped
  * (B2_DEVERR_BLOCK_ID).

@@ -18,8 +18,9 @@
 //     head (up to 8 columns).  S = sum_g s_g (A q)_g + sum_g (m_g - 8 s_g) Q_g, Q_g the
 //     group's sum of q; the first sum is taken in fp32, the second is one more
 //     product whose columns are m and s and whose B is Q in two f16 parts.
-//     q is scaled by a power of two to at most 2^9, so its f16 form is exact
-//     down to 2^-23 of the row's largest element.
+//     q is scaled by a power of two to at most 2^9 (and a sixteenth of it where the code
+//     counts 16 times): its f16 form is exact down to 2^-19 of the row's largest element
+//     (f16; bf16 2^-22), and off by 2^-29 of that element at most below.
 //   * Values: A = V codes transposed (16 dims x 16 tokens), B = f16(p s 2^k), k per
 //     group of 32 dims; C adds up sum p s c.  The f16 rounding of p s would count
 //     with c up to 15; adding the same product with A = -8 makes it count with

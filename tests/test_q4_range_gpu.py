@@ -281,3 +281,28 @@ def test_values_at_the_ends_of_f16s_range(b2, cuda, dt, dim, group, size):
     got = _attend(b2, dt, pool, q_bits, tables, lens, group=group, out_dtype=torch.float32)[0]
     _check(got, want, bound + 100 * 2.0 ** -45, dt, True)
     assert b2.device_errors() == 0
+
+
+@pytest.mark.parametrize("ratio", [8, 14, 20])
+@pytest.mark.parametrize("dt", [R.F16, R.BF16])
+def test_queries_with_one_huge_element(b2, cuda, dt, ratio):
+    """One element of q 2^ratio times the others, at a dim whose keys are 0 (their group's step is 0 too): the others, kept to 2^-29 of it,
+    make the scores."""
+    torch = _torch()
+    rng = _rng(ratio)
+    dim, n = 64, 200
+    tables, blocks = tables_for(rng, [n])
+    pool = _filled(rng, blocks, 1, 1, dim, k_spread=np.where(np.arange(dim) < 32, 0.0, 1.0))
+    q_bits, q = rows16(rng, dt, (1, 4, dim), 2.0 ** -6)
+    q[:, :, 5] = 2.0 ** (ratio - 6)
+    q_bits = R.O.round_to(dt, q.astype(np.float32).ravel()).reshape(q.shape)
+    q = R.widen(dt, q_bits)
+    want, bound = _want(pool, q, tables, [n], group=4, scale=8.0)
+    k, v, ks, km, vs, vm = pool.rows(tables[0][np.arange(n) // 16].astype(np.int64) * 16 + np.arange(n) % 16, 0)
+    err = 8.0 * 2.0 ** (ratio - 6 - 29) * (32 * (8 * ks[:, 0] + np.abs(km[:, 0]))).sum(-1).max()  # of a score
+    bound += 2 * err * np.abs(v).max()
+    got = _attend(b2, dt, pool, q_bits, tables, np.array([n], np.int32), group=4, scale=8.0, out_dtype=torch.float32)[0]
+    _check(got, want, bound, dt, True)
+    # The bound is not idle: at 2^20 a score may be off by 8 2^-15 32 (8 s + |m|) = 0.029 with s up to 0.4 and |m| up to 0.5 in
+    # one group, an output by twice that times the largest value, 3.9: 0.23.  It falls with the ratio.
+    assert bound.max() < 0.1 * np.abs(v).max()
