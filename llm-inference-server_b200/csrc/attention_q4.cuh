@@ -206,8 +206,8 @@ struct Q4State {
 };
 
 // The scale word of a k from -7 to 25: s 2^k < 2^11 below the limit (an f16's exponent bits, 26 - k), and the factor
-// exactly (a subnormal f16 below k = -3).  A step that equals the limit and passes it by its middle's bits alone is
-// taken as below it: 2^11, with weights of up to 2^4 still in f16's range.
+// exactly (a subnormal f16 below k = -3).  A step of just 2^(11 - k) may count as below the limit (the words' low halves
+// decide): with p <= 2^4 its product is still in f16's range.
 __device__ __forceinline__ uint32_t q4_scale(int k) {
     const int e = k - kQ4Weight;
     return static_cast<uint32_t>(26 - k) << 26 | static_cast<uint32_t>(e >= -14 ? (e + 15) << 10 : 1 << (e + 24));

@@ -65,8 +65,8 @@ __device__ __forceinline__ uint32_t q4_codes_exact(const float (&x)[8], float m,
 // most, which puts the range's upper end at 7.01; a subnormal s may be off by half of itself and the end
 // at 14.5) and m's own rounding (2^-11 |m|) is under 0.45 s; elsewhere limit is 0.  What is not within it -- 0.06 %
 // of the elements of normal bf16 rows, mostly exact ties; groups far from zero for their width; steps
-// below 2^-14; saturated groups -- takes the definition.  Four codes are added up as c0 + 16 c1 + 256 c2 + 4096 c3 in fp32 (exact): fp32 instructions
-// issue at twice the integer ones' rate.
+// below 2^-14; saturated groups -- takes the definition.  Four codes are added up as c0 + 16 c1 + 256 c2 +
+// 4096 c3 in fp32 (exact): fp32 instructions issue at twice the integer ones' rate.
 __device__ __forceinline__ uint32_t q4_codes(const float (&x)[8], float m, float s, float rs, float ms, float limit) {
     constexpr float kMagic = 12582912.0f;  // 1.5 2^23: adding it rounds to an integer, ties to even
     float far = 0.0f, packed[2];
